@@ -45,6 +45,22 @@ class axkv_cache_t(C.Structure):
     ]
 
 
+class axkv4_cache_t(C.Structure):
+    _fields_ = [
+        ("pages", C.c_void_p), ("block_table", C.c_void_p), ("n_seqs", C.c_int32),
+        ("max_blocks", C.c_int32), ("n_pages", C.c_int32), ("n_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("page_tokens", C.c_int32),
+    ]
+
+
+class axkv_pages_t(C.Structure):
+    _fields_ = [
+        ("block_table", C.c_void_p), ("ref_count", C.c_void_p), ("pools", C.c_void_p),
+        ("page_bytes", C.c_int64), ("n_pools", C.c_int32), ("n_seqs", C.c_int32),
+        ("max_blocks", C.c_int32), ("n_pages", C.c_int32),
+    ]
+
+
 class axdec_config_t(C.Structure):
     _fields_ = [
         ("n_layers", C.c_int32), ("hidden", C.c_int32), ("ffn", C.c_int32),
@@ -102,6 +118,21 @@ SIGNATURES: dict[str, tuple] = {
                                       _P]),
     "axkv_paged_prefill_attn": (_I32, [C.POINTER(axkv_cache_t), _P, _I64, _I32, _I32, _I32, _I32,
                                        _P, _P, _P, _P]),
+    "axkv4_pages_bytes": (_I64, [C.POINTER(axkv4_cache_t)]),
+    "axkv4_append": (_I32, [C.POINTER(axkv4_cache_t), _P, _P, _I64, _I32, _P, _P, _P]),
+    "axkv4_read": (_I32, [C.POINTER(axkv4_cache_t), _P, _P, _I64, _I32, _P, _P, _P]),
+    "axkv4_decode_attn_workspace": (_I64, [C.POINTER(axkv4_cache_t), _I32, _I32]),
+    "axkv4_decode_attn": (_I32, [C.POINTER(axkv4_cache_t), _P, _I64, _I32, _I32, _P, _P, _P, _P,
+                                 _I64, _P]),
+    "axkv4_chunk_attn_workspace": (_I64, [C.POINTER(axkv4_cache_t), _I32, _I32, _I32]),
+    "axkv4_chunk_attn": (_I32, [C.POINTER(axkv4_cache_t), _P, _I64, _I32, _I32, _I32, _I32, _P, _P,
+                                _P, _P, _P, _I64, _P]),
+    "axkv_pages_workspace": (_I64, [C.POINTER(axkv_pages_t), _I32]),
+    "axkv_pages_reserve": (_I32, [C.POINTER(axkv_pages_t), _P, _P, _I32, _P, _I64, _P]),
+    "axkv_pages_fork": (_I32, [C.POINTER(axkv_pages_t), _P, _P, _P, _I32, _P, _I64, _P]),
+    "axkv_pages_free": (_I32, [C.POINTER(axkv_pages_t), _P, _I32, _P]),
+    "axkv_pages_compact": (_I32, [C.POINTER(axkv_pages_t), _P, _P, _I64, _P]),
+    "axkv_pages_copy": (_I32, [C.POINTER(axkv_pages_t), _P, _P, _I32, _P]),
     "axtp_allreduce_sum": (_I32, [_P, _I64, _P]),
     "axdec_tp_allreduce_kind": (_I32, [_P]),
     "axdec_tp_health": (_I32, [_P, C.POINTER(C.c_int), C.POINTER(C.c_int)]),

@@ -9,6 +9,7 @@ sequence s owns pages s * max_blocks onwards (identity block table).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -127,3 +128,233 @@ class PagedKVCache:
                                                 C.c_void_p(out.data_ptr()), None, None,
                                                 self._stream()))
         return out
+
+
+def _on(device: torch.device):
+    """The device of the cache as the current one, for the length of a call."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index \
+        else torch.cuda.device(device)
+
+
+class PagedKVCache4:
+    """The paged cache in 4 bits (include/axkv.h, axkv4_cache): K and V as 4-bit
+    codes with a step and a zero point per token and 32 dims, 0.5625 byte per
+    value, under the method names of :class:`PagedKVCache`.
+
+    Without arguments of its own the cache is one layer of ``max_seqs``
+    sequences with an identity block table.  ``pages`` (uint8 [n_pages,
+    n_kv_heads, 18 * head_dim]) and ``block_table`` (int32 [sequences,
+    max_blocks], -1: no page) make it a view of a caller's memory, e.g. one
+    layer of a pool whose table a :class:`~axion_b200.kv_pages.KVPages`
+    manages; sequences and positions are then named by the caller
+    (``append_rows``, ``decode_attention``, ``chunk_attention``).
+
+    Calls go to the current stream of the cache's device; calls of one cache
+    on several streams have their own workspaces, and so has every captured
+    graph.
+    """
+
+    page_size = 16
+
+    def __init__(self, n_kv_heads: int, head_dim: int, max_seqs: int = 1, max_tokens: int = 4096,
+                 device=None, *, pages: torch.Tensor | None = None,
+                 block_table: torch.Tensor | None = None):
+        if head_dim not in (32, 64, 128):
+            raise RuntimeError(f"PagedKVCache4: head_dim {head_dim} (32, 64, 128)")
+        if n_kv_heads <= 0 or max_seqs <= 0 or max_tokens <= 0:
+            raise RuntimeError("PagedKVCache4: sizes must be positive")
+        self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
+        self.hidden_size = n_kv_heads * head_dim
+        if (pages is None) != (block_table is None):
+            raise RuntimeError("PagedKVCache4: pages and block_table come together")
+        if pages is None:
+            dev = torch.device(device) if device is not None else torch.device("cuda")
+            blocks = (max_tokens + self.page_size - 1) // self.page_size
+            pages = torch.zeros(max_seqs * blocks, n_kv_heads, 18 * head_dim, dtype=torch.uint8,
+                                device=dev)
+            block_table = torch.arange(max_seqs * blocks, dtype=torch.int32,
+                                       device=dev).view(max_seqs, blocks)
+        if not pages.is_cuda or block_table.device != pages.device:
+            raise RuntimeError("PagedKVCache4: pages and block_table must be CUDA tensors of one "
+                               "device (axion_b200 has no CPU path)")
+        if (pages.dtype != torch.uint8 or pages.dim() != 3 or not pages.is_contiguous()
+                or tuple(pages.shape[1:]) != (n_kv_heads, 18 * head_dim) or pages.shape[0] == 0):
+            raise RuntimeError(f"PagedKVCache4: pages must be contiguous uint8 [n_pages, "
+                               f"{n_kv_heads}, {18 * head_dim}]")
+        if (block_table.dtype != torch.int32 or block_table.dim() != 2
+                or not block_table.is_contiguous() or block_table.numel() == 0):
+            raise RuntimeError("PagedKVCache4: block_table must be contiguous int32 [sequences, "
+                               "max_blocks]")
+        self.pages, self.block_table = pages, block_table
+        self.max_seqs, self.max_blocks = block_table.shape
+        self.used = [0] * self.max_seqs
+        self.c = _lib.axkv4_cache_t(pages.data_ptr(), block_table.data_ptr(), self.max_seqs,
+                                    self.max_blocks, pages.shape[0], n_kv_heads, head_dim,
+                                    self.page_size)
+        self._ref = C.byref(self.c)
+        self._ws: dict[int, torch.Tensor] = {}
+        self._need: dict[tuple, int] = {}
+        self._lib = _lib.load()
+
+    # -- arguments ---------------------------------------------------------------
+    def _ints(self, t: torch.Tensor | None, n: int, what: str) -> int | None:
+        if t is None:
+            return None
+        if t.dtype != torch.int32 or t.device != self.pages.device or t.dim() != 1 \
+                or t.shape[0] != n or not t.is_contiguous():
+            raise RuntimeError(f"PagedKVCache4: {what} must be contiguous int32 [{n}] on the "
+                               "cache's device")
+        return t.data_ptr()
+
+    def _rows(self, t: torch.Tensor, width: int, what: str) -> torch.Tensor:
+        """fp32 rows [n, width], 16-byte aligned, with a row pitch the kernels take."""
+        if t.dim() != 2 or t.shape[1] != width or t.device != self.pages.device:
+            raise RuntimeError(f"PagedKVCache4: {what} must be [rows, {width}] on the cache's device")
+        if t.dtype != torch.float32:
+            t = t.float()
+        if t.shape[0] and (t.stride(1) != 1 or t.stride(0) % 4 or t.stride(0) < width
+                           or t.data_ptr() % 16):
+            t = t.clone(memory_format=torch.contiguous_format)
+        return t
+
+    def _out(self, out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+        if out is None:
+            return torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        if out.shape != q.shape or out.dtype != torch.float32 or out.device != q.device \
+                or not out.is_contiguous() or out.data_ptr() % 16:
+            raise RuntimeError("PagedKVCache4: out must be contiguous fp32 like q, 16-byte aligned")
+        return out
+
+    def _workspace(self, fn, *sizes: int) -> torch.Tensor:
+        key = (fn.__name__, *sizes)
+        need = self._need.get(key)
+        if need is None:
+            need = self._need[key] = fn(self._ref, *sizes)
+        if need < 0:
+            raise RuntimeError(_lib.load().axq8_last_error().decode(errors="replace")
+                               or "PagedKVCache4: unsupported attention shape")
+        if torch.cuda.is_current_stream_capturing():
+            # a graph keeps its own: it may be replayed beside any other call
+            return torch.zeros(need, dtype=torch.uint8, device=self.pages.device)
+        stream = torch.cuda.current_stream(self.pages.device).cuda_stream
+        ws = self._ws.get(stream)
+        if ws is None or ws.numel() < need:
+            ws = self._ws[stream] = torch.zeros(need, dtype=torch.uint8, device=self.pages.device)
+        return ws
+
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.pages.device).cuda_stream
+
+    # -- rows of a caller's sequences ----------------------------------------------
+    def append_rows(self, K: torch.Tensor, V: torch.Tensor, row_seq: torch.Tensor,
+                    row_pos: torch.Tensor) -> None:
+        """K, V rows [n, hidden] (fp32, device) to positions row_pos of sequences
+        row_seq (int32 [n], device), no position twice."""
+        K, V = self._rows(K, self.hidden_size, "K"), self._rows(V, self.hidden_size, "V")
+        n = K.shape[0]
+        if V.shape[0] != n:
+            raise RuntimeError("PagedKVCache4: K and V must be [rows, hidden]")
+        if n and K.stride(0) != V.stride(0):
+            K, V = K.contiguous(), V.contiguous()
+        seq, pos = self._ints(row_seq, n, "row_seq"), self._ints(row_pos, n, "row_pos")
+        with _on(self.pages.device):
+            check(self._lib.axkv4_append(self._ref, K.data_ptr(), V.data_ptr(),
+                                         K.stride(0) if n else self.hidden_size, n, seq, pos,
+                                         self._stream()))
+
+    def read_rows(self, row_seq: torch.Tensor, row_pos: torch.Tensor):
+        """The values held at those positions: (K, V) fp32 [n, hidden]."""
+        n = row_seq.shape[0]
+        seq, pos = self._ints(row_seq, n, "row_seq"), self._ints(row_pos, n, "row_pos")
+        kv = torch.empty(2, n, self.hidden_size, dtype=torch.float32, device=self.pages.device)
+        with _on(self.pages.device):
+            check(self._lib.axkv4_read(self._ref, kv[0].data_ptr(), kv[1].data_ptr(),
+                                       self.hidden_size, n, seq, pos, self._stream()))
+        return kv[0], kv[1]
+
+    def decode_attention(self, q: torch.Tensor, n_heads: int, q_pos: torch.Tensor,
+                         q_seq: torch.Tensor | None = None, out: torch.Tensor | None = None):
+        """Attention of row r of q [n, n_heads * head_dim] (fp32, device), at
+        position q_pos[r] of sequence q_seq[r] (None: sequence r), over tokens
+        0 .. q_pos[r]; rows at negative positions give zeros."""
+        q = self._rows(q, n_heads * self.head_dim, "q")
+        n = q.shape[0]
+        out = self._out(out, q)
+        pos, seq = self._ints(q_pos, n, "q_pos"), self._ints(q_seq, n, "q_seq")
+        if n == 0:
+            return out
+        with _on(self.pages.device):
+            ws = self._workspace(self._lib.axkv4_decode_attn_workspace, n, n_heads)
+            check(self._lib.axkv4_decode_attn(self._ref, q.data_ptr(), q.stride(0), n, n_heads, seq,
+                                              pos, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                              self._stream()))
+        return out
+
+    def chunk_attention(self, q: torch.Tensor, n_heads: int, q_start: torch.Tensor,
+                        q_pos: torch.Tensor, max_rows: int, q_seq: torch.Tensor | None = None,
+                        out: torch.Tensor | None = None):
+        """Causal attention of ragged chunks: rows q_start[i] .. q_start[i + 1] - 1
+        of q are sequence q_seq[i] (None: sequence i) at positions q_pos[i] and
+        on, at most max_rows of them, their K and V appended.  Rows of no chunk
+        are left as they are in `out` (unset where it is made here)."""
+        q = self._rows(q, n_heads * self.head_dim, "q")
+        n, chunks = q.shape[0], q_pos.shape[0]
+        out = self._out(out, q)
+        start = self._ints(q_start, chunks + 1, "q_start")
+        pos, seq = self._ints(q_pos, chunks, "q_pos"), self._ints(q_seq, chunks, "q_seq")
+        if n == 0 or chunks == 0 or max_rows == 0:
+            return out
+        with _on(self.pages.device):
+            ws = self._workspace(self._lib.axkv4_chunk_attn_workspace, chunks, max_rows, n_heads)
+            check(self._lib.axkv4_chunk_attn(self._ref, q.data_ptr(), q.stride(0), n, chunks,
+                                             max_rows, n_heads, seq, start, pos, out.data_ptr(),
+                                             ws.data_ptr(), ws.numel(), self._stream()))
+        return out
+
+    # -- the reference's names, sequences filled from their start -------------------
+    def initialize(self, hidden: int, page: int = 16) -> None:
+        """PagedKVCache::initialize: empties the cache."""
+        if hidden != self.hidden_size or page != self.page_size:
+            raise RuntimeError(f"PagedKVCache: hidden {hidden} / page {page} do not match "
+                               f"{self.hidden_size} / {self.page_size}")
+        self.used = [0] * self.max_seqs
+
+    def _span(self, seq: int, a: int, b: int):
+        dev = self.pages.device
+        return (torch.full((b - a,), seq, dtype=torch.int32, device=dev),
+                torch.arange(a, b, dtype=torch.int32, device=dev))
+
+    def append(self, K: torch.Tensor, V: torch.Tensor, seq: int = 0) -> None:
+        """Append rows K, V [rows, hidden] (fp32, device) to sequence `seq`."""
+        if K.shape != V.shape or K.dim() != 2 or K.shape[1] != self.hidden_size:
+            raise RuntimeError("PagedKVCache::append: K and V must be [rows, hidden]")
+        n = self.used[seq] + K.shape[0]
+        if n > self.max_blocks * self.page_size:
+            raise RuntimeError("PagedKVCache::append: sequence full")
+        self.append_rows(K, V, *self._span(seq, self.used[seq], n))
+        self.used[seq] = n
+
+    def materialize_keys(self, seq: int = 0) -> torch.Tensor:
+        return self.read_rows(*self._span(seq, 0, self.used[seq]))[0]
+
+    def materialize_values(self, seq: int = 0) -> torch.Tensor:
+        return self.read_rows(*self._span(seq, 0, self.used[seq]))[1]
+
+    def attention(self, q: torch.Tensor, n_heads: int) -> torch.Tensor:
+        """Decode attention of one query row per sequence over all its tokens."""
+        if q.shape[0] > self.max_seqs or min(self.used[:q.shape[0]], default=1) <= 0:
+            raise RuntimeError("PagedKVCache: attention over an empty sequence")
+        pos = torch.tensor(self.used[:q.shape[0]], dtype=torch.int32, device=self.pages.device) - 1
+        return self.decode_attention(q, n_heads, pos)
+
+    def prefill_attention(self, q: torch.Tensor, n_heads: int, T: int, p0: int) -> torch.Tensor:
+        """Causal attention of positions p0 .. p0 + T - 1 of every sequence (row
+        s * T + t = sequence s, position p0 + t), their K/V already appended."""
+        n_seq = q.shape[0] // T if T > 0 else 0
+        if n_seq * T != q.shape[0] or n_seq > self.max_seqs \
+                or any(self.used[s] < p0 + T for s in range(n_seq)):
+            raise RuntimeError("PagedKVCache: prefill rows must be appended first")
+        dev = self.pages.device
+        return self.chunk_attention(
+            q, n_heads, torch.arange(n_seq + 1, dtype=torch.int32, device=dev) * T,
+            torch.full((n_seq,), p0, dtype=torch.int32, device=dev), T)
