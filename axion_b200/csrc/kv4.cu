@@ -12,17 +12,12 @@
 #include "axkv.h"
 #include "common.cuh"
 #include "kv4.cuh"
+#include "kv4_narrow.cuh"
 #include "runtime.h"
 
 using namespace axq8;
 
 namespace {
-
-struct Kv4Pages {
-    uint8_t* pages;
-    const int* table;
-    int n_seqs, max_blocks, n_pages, n_kv;
-};
 
 // The page of position p of sequence s, or null outside the table or the pool.
 template <int HD>
@@ -114,65 +109,6 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Attention, one warp per (query row, head): one pass over the tokens with the
-// running maximum and sum of the softmax; lane l holds dims 32 b + l.
-// Rows of chunk i (start null: row i alone) sit at positions q_pos[i] ...
-template <int HD>
-__global__ void __launch_bounds__(256)
-    kv4_attn_rows_kernel(Kv4Pages c, const float* __restrict__ q, int64_t ldq, int n_rows,
-                         int max_rows, int n_heads, const int* __restrict__ q_seq,
-                         const int* __restrict__ q_start, const int* __restrict__ q_pos, float scale,
-                         float* __restrict__ out, int* __restrict__ status) {
-    constexpr int NB = Kv4<HD>::NB;
-    const int lane = threadIdx.x & 31;
-    const int h = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int j = blockIdx.y, i = blockIdx.z;
-    if (h >= n_heads) return;
-    int row = i;
-    if (q_start) {
-        row = q_start[i] + j;
-        const int end = q_start[i + 1];
-        if (end - q_start[i] > max_rows || end > n_rows || q_start[i] < 0) {
-            if (lane == 0) record_status(status, AXQ8_ERR_INVALID);
-            if (row < 0 || row >= n_rows) return;
-        }
-        if (row >= end) return;
-    }
-    const int seq = q_seq ? q_seq[i] : i;
-    int ctx = q_pos[i] + j + 1;
-    if (seq < 0 || seq >= c.n_seqs || ctx > c.max_blocks * kKv4Tokens) {
-        if (lane == 0) record_status(status, AXQ8_ERR_INVALID);
-        ctx = seq < 0 || seq >= c.n_seqs ? 0 : c.max_blocks * kKv4Tokens;
-    }
-    float qv[NB], acc[NB], m = -CUDART_INF_F, l = 0.0f;
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-        qv[b] = q[(int64_t)row * ldq + (int64_t)h * HD + 32 * b + lane];
-        acc[b] = 0.0f;
-    }
-    for (int p = 0; p < ctx; p++) {
-        const uint8_t* base = kv4_at<HD>(c, seq, p, h / (n_heads / c.n_kv));
-        if (!base) {
-            if (lane == 0) record_status(status, AXQ8_ERR_INVALID);
-            continue;
-        }
-        float dot = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-            dot = fmaf(qv[b], kv4_value<HD>(base, false, p % kKv4Tokens, b, lane), dot);
-        const float s = warp_sum(dot) * scale;
-        const float mn = fmaxf(m, s), corr = expf(m - mn), e = expf(s - mn);
-        l = fmaf(l, corr, e);
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-            acc[b] = fmaf(e, kv4_value<HD>(base, true, p % kKv4Tokens, b, lane), acc[b] * corr);
-        m = mn;
-    }
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-        out[(int64_t)row * n_heads * HD + (int64_t)h * HD + 32 * b + lane] = l > 0.0f ? acc[b] / l : 0.0f;
-}
-
 int check_cache4(const axkv4_cache_t* c, const char* what) {
     if (!c || !c->pages || !c->block_table) return fail(AXQ8_ERR_INVALID, "%s: null cache pointer", what);
     if (c->page_tokens != kKv4Tokens)
@@ -238,13 +174,64 @@ cudaError_t launch_read(const axkv4_cache_t* c, float* k, float* v, int64_t ld, 
                     pages_of(c), k, v, ld, n_rows, seq, pos, status);
 }
 
+// How the columns of a KV head are tiled and the context split.
+struct NarrowPlan {
+    int nt, tiles, nsplit;   // n-tiles of 8 columns, column tiles per (chunk, KV head), splits
+    int64_t counters, workspace;   // bytes
+};
+
+// About three CTAs per SM and wave; a split is at least kNarrowMinPages.
+NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int chunks, int rows, int G) {
+    NarrowPlan p;
+    const int cols = rows * G;
+    p.nt = cols <= 8 ? 1 : 2;
+    p.tiles = (cols + 8 * p.nt - 1) / (8 * p.nt);
+    const int64_t ctas = (int64_t)c->n_kv_heads * p.tiles * chunks;
+    const int most = std::min(kNarrowMaxSplits, (c->max_blocks + kNarrowMinPages - 1) / kNarrowMinPages);
+    const int64_t want = 6ll * ds->sm_count;
+    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(most, (want + ctas - 1) / ctas));
+    // split calls have fewer than `want` tiles: a counter for each in front, in the same
+    // place for calls of every size, then the partials
+    p.counters = (want * 4 + 15) / 16 * 16;
+    p.workspace = p.counters + (p.nsplit > 1 ? ctas * p.nsplit * 8 * p.nt * (c->head_dim + 2) * 4 : 0);
+    return p;
+}
+
+template <int HD, int NT>
+cudaError_t launch_narrow_nt(const NarrowArgs& a, dim3 grid, cudaStream_t s) {
+    constexpr size_t smem = NarrowCfg<HD, NT>::SMEM;
+    auto kern = kv4_attn_narrow_kernel<HD, NT>;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_k(kern, grid, dim3(kNarrowWarps * 32), smem, s, false, a);
+}
+
 template <int HD>
-cudaError_t launch_rows(const axkv4_cache_t* c, const float* q, int64_t ldq, int n_rows, int chunks,
-                        int max_rows, int n_heads, const int* q_seq, const int* q_start,
-                        const int* q_pos, float* out, int* status, cudaStream_t s) {
-    return launch_k(kv4_attn_rows_kernel<HD>, dim3((n_heads + 7) / 8, max_rows, chunks), dim3(256), 0, s,
-                    false, pages_of(c), q, ldq, n_rows, max_rows, n_heads, q_seq, q_start, q_pos,
-                    1.0f / std::sqrt((float)HD), out, status);
+cudaError_t launch_narrow(const NarrowPlan& p, const axkv4_cache_t* c, const float* q, int64_t ldq,
+                          int n_rows, int chunks, int max_rows, int n_heads, const int* q_seq,
+                          const int* q_start, const int* q_pos, float* out, void* ws, int* status,
+                          cudaStream_t s) {
+    NarrowArgs a = {};
+    a.c = pages_of(c);
+    a.q = q;
+    a.ldq = ldq;
+    a.n_rows = n_rows;
+    a.max_rows = max_rows;
+    a.n_heads = n_heads;
+    a.G = n_heads / c->n_kv_heads;
+    a.nsplit = p.nsplit;
+    a.q_seq = q_seq;
+    a.q_start = q_start;
+    a.q_pos = q_pos;
+    a.scale = 1.4426950408889634f / std::sqrt((float)HD);
+    a.out = out;
+    a.counters = static_cast<int*>(ws);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.counters);
+    a.status = status;
+    const dim3 grid(c->n_kv_heads * p.tiles, chunks, p.nsplit);
+    return p.nt == 1 ? launch_narrow_nt<HD, 1>(a, grid, s) : launch_narrow_nt<HD, 2>(a, grid, s);
 }
 
 }  // namespace
@@ -282,7 +269,9 @@ int axkv4_read(const axkv4_cache_t* c, float* k_rows, float* v_rows, int64_t ld,
 
 int64_t axkv4_decode_attn_workspace(const axkv4_cache_t* c, int32_t n_rows, int32_t n_heads) {
     if (check_attn(c, "axkv4_decode_attn_workspace", n_heads) || n_rows <= 0) return -1;
-    return 16;
+    DeviceState* ds = device_state();
+    if (!ds) return -1;
+    return narrow_plan(ds, c, n_rows, 1, n_heads / c->n_kv_heads).workspace;
 }
 
 int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_t n_rows,
@@ -299,12 +288,16 @@ int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32
         return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: q, out and workspace must be 16-byte aligned");
     if (!q_seq && n_rows > c->n_seqs)
         return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: %d rows of %d sequences", n_rows, c->n_seqs);
-    if (workspace_bytes < axkv4_decode_attn_workspace(c, n_rows, n_heads))
-        return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: workspace %lld B", (long long)workspace_bytes);
+    if (workspace_bytes <= 0) return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: no workspace");
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
-    AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_rows, c, q, ldq, n_rows, n_rows, 1, n_heads, q_seq,
-                                  nullptr, q_pos, out, ds->status, static_cast<cudaStream_t>(stream)),
+    const NarrowPlan p = narrow_plan(ds, c, n_rows, 1, n_heads / c->n_kv_heads);
+    if (workspace_bytes < p.workspace)
+        return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: workspace %lld B < %lld B",
+                    (long long)workspace_bytes, (long long)p.workspace);
+    AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_narrow, p, c, q, ldq, n_rows, n_rows, 1, n_heads,
+                                  q_seq, nullptr, q_pos, out, workspace, ds->status,
+                                  static_cast<cudaStream_t>(stream)),
                   "axkv4_decode_attn launch");
     return AXQ8_OK;
 }
@@ -312,7 +305,9 @@ int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32
 int64_t axkv4_chunk_attn_workspace(const axkv4_cache_t* c, int32_t n_chunks, int32_t max_rows,
                                    int32_t n_heads) {
     if (check_attn(c, "axkv4_chunk_attn_workspace", n_heads) || n_chunks <= 0 || max_rows <= 0) return -1;
-    return 16;
+    DeviceState* ds = device_state();
+    if (!ds) return -1;
+    return narrow_plan(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads).workspace;
 }
 
 int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_t n_rows,
@@ -333,12 +328,17 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
         return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: q, out and workspace must be 16-byte aligned");
     if (!q_seq && n_chunks > c->n_seqs)
         return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: %d chunks of %d sequences", n_chunks, c->n_seqs);
-    if (workspace_bytes < axkv4_chunk_attn_workspace(c, n_chunks, max_rows, n_heads))
-        return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: workspace %lld B", (long long)workspace_bytes);
+    if (workspace_bytes <= 0) return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: no workspace");
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
-    AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_rows, c, q, ldq, n_rows, n_chunks, max_rows, n_heads,
-                                  q_seq, q_start, q_pos, out, ds->status,
+    const NarrowPlan p = narrow_plan(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads);
+    if (workspace_bytes < p.workspace)
+        return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: workspace %lld B < %lld B",
+                    (long long)workspace_bytes, (long long)p.workspace);
+    if ((int64_t)p.tiles * c->n_kv_heads > 0x7fffffff)
+        return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d rows of %d heads", max_rows, n_heads);
+    AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_narrow, p, c, q, ldq, n_rows, n_chunks, max_rows,
+                                  n_heads, q_seq, q_start, q_pos, out, workspace, ds->status,
                                   static_cast<cudaStream_t>(stream)),
                   "axkv4_chunk_attn launch");
     return AXQ8_OK;
