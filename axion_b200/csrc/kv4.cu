@@ -174,38 +174,44 @@ cudaError_t launch_read(const axkv4_cache_t* c, float* k, float* v, int64_t ld, 
                     pages_of(c), k, v, ld, n_rows, seq, pos, status);
 }
 
-// How the columns of a KV head are tiled and the context split.
+// Columns of a tile, CTAs, and workspace bytes: a record per CTA, then two
+// partial states per CTA.
 struct NarrowPlan {
-    int nt, tiles, nsplit;   // n-tiles of 8 columns, column tiles per (chunk, KV head), splits
-    int64_t counters, workspace;   // bytes
+    int cols, ctas, aligned;
+    int64_t records, workspace;
+    int64_t units;   // of work, at most
 };
 
-// About three CTAs per SM and wave; a split is at least kNarrowMinPages.
-NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int chunks, int rows, int G) {
+NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int entries, int rows, int G) {
     NarrowPlan p;
-    const int cols = rows * G;
-    p.nt = cols <= 8 ? 1 : 2;
-    p.tiles = (cols + 8 * p.nt - 1) / (8 * p.nt);
-    const int64_t ctas = (int64_t)c->n_kv_heads * p.tiles * chunks;
-    const int most = std::min(kNarrowMaxSplits, (c->max_blocks + kNarrowMinPages - 1) / kNarrowMinPages);
-    const int64_t want = 6ll * ds->sm_count;
-    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(most, (want + ctas - 1) / ctas));
-    // split calls have fewer than `want` tiles: a counter for each in front, in the same
-    // place for calls of every size, then the partials
-    p.counters = (want * 4 + 15) / 16 * 16;
-    p.workspace = p.counters + (p.nsplit > 1 ? ctas * p.nsplit * 8 * p.nt * (c->head_dim + 2) * 4 : 0);
+    const int64_t cols = (int64_t)rows * G;
+    p.cols = cols <= 4 ? 4 : cols <= 8 ? 8 : 16;
+    const int slots = ds->sm_count * (p.cols == 4 ? 4 : p.cols == 8 ? 3 : 2);
+    const int64_t tiles = (cols + p.cols - 1) / p.cols * c->n_kv_heads * entries;
+    // every tile starts a run where that leaves half of the runs; with the most
+    // tiles a call can have (it may have fewer), this many runs are never exceeded
+    p.aligned = 2 * tiles <= slots ? (int)tiles : 0;
+    const int64_t runs = (tiles * c->max_blocks + kNarrowMinPages - 1) / kNarrowMinPages + p.aligned;
+    p.ctas = (int)std::min<int64_t>(slots, runs);
+    p.units = tiles * (c->max_blocks + kNarrowTileCost) * 2;
+    p.records = ((int64_t)p.ctas * sizeof(NarrowPart) + 15) / 16 * 16;
+    p.workspace = p.records + (int64_t)p.ctas * 2 * p.cols * (c->head_dim + 2) * 4;
     return p;
 }
 
-template <int HD, int NT>
-cudaError_t launch_narrow_nt(const NarrowArgs& a, dim3 grid, cudaStream_t s) {
-    constexpr size_t smem = NarrowCfg<HD, NT>::SMEM;
-    auto kern = kv4_attn_narrow_kernel<HD, NT>;
+template <int HD, int COLS>
+cudaError_t launch_narrow_cols(const NarrowArgs& a, int ctas, cudaStream_t s) {
+    static_assert(NarrowCfg<HD, COLS>::CTAS == (COLS == 4 ? 4 : COLS == 8 ? 3 : 2), "narrow_plan");
+    constexpr size_t smem = NarrowCfg<HD, COLS>::SMEM;
+    auto kern = kv4_attn_narrow_kernel<HD, COLS>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    return launch_k(kern, grid, dim3(kNarrowWarps * 32), smem, s, false, a);
+    const cudaError_t e = launch_k(kern, dim3(ctas), dim3(kNarrowWarps * 32), smem, s, false, a);
+    if (e != cudaSuccess) return e;
+    constexpr int blocks = COLS * HD / 4 / NarrowCfg<HD, COLS>::JOIN_ITEMS;
+    return launch_k(kv4_attn_join_kernel<HD, COLS>, dim3(ctas, blocks), dim3(kJoinThreads), 0, s, true, a);
 }
 
 template <int HD>
@@ -221,17 +227,19 @@ cudaError_t launch_narrow(const NarrowPlan& p, const axkv4_cache_t* c, const flo
     a.max_rows = max_rows;
     a.n_heads = n_heads;
     a.G = n_heads / c->n_kv_heads;
-    a.nsplit = p.nsplit;
+    a.n_entries = chunks;
+    a.aligned = p.aligned;
     a.q_seq = q_seq;
     a.q_start = q_start;
     a.q_pos = q_pos;
     a.scale = 1.4426950408889634f / std::sqrt((float)HD);
     a.out = out;
-    a.counters = static_cast<int*>(ws);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.counters);
+    a.split = static_cast<NarrowPart*>(ws);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.records);
     a.status = status;
-    const dim3 grid(c->n_kv_heads * p.tiles, chunks, p.nsplit);
-    return p.nt == 1 ? launch_narrow_nt<HD, 1>(a, grid, s) : launch_narrow_nt<HD, 2>(a, grid, s);
+    return p.cols == 4   ? launch_narrow_cols<HD, 4>(a, p.ctas, s)
+           : p.cols == 8 ? launch_narrow_cols<HD, 8>(a, p.ctas, s)
+                         : launch_narrow_cols<HD, 16>(a, p.ctas, s);
 }
 
 }  // namespace
@@ -292,6 +300,8 @@ int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
     const NarrowPlan p = narrow_plan(ds, c, n_rows, 1, n_heads / c->n_kv_heads);
+    if (p.units > 0x7fffffff)
+        return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_decode_attn: %d rows of %d pages", n_rows, c->max_blocks);
     if (workspace_bytes < p.workspace)
         return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: workspace %lld B < %lld B",
                     (long long)workspace_bytes, (long long)p.workspace);
@@ -332,11 +342,12 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
     const NarrowPlan p = narrow_plan(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads);
+    if (p.units > 0x7fffffff)
+        return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d chunks of %d rows, %d pages", n_chunks,
+                    max_rows, c->max_blocks);
     if (workspace_bytes < p.workspace)
         return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: workspace %lld B < %lld B",
                     (long long)workspace_bytes, (long long)p.workspace);
-    if ((int64_t)p.tiles * c->n_kv_heads > 0x7fffffff)
-        return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d rows of %d heads", max_rows, n_heads);
     AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_narrow, p, c, q, ldq, n_rows, n_chunks, max_rows,
                                   n_heads, q_seq, q_start, q_pos, out, workspace, ds->status,
                                   static_cast<cudaStream_t>(stream)),

@@ -1,7 +1,7 @@
 // Attention of few columns over the 4-bit cache: decode steps and short chunks.
 //
-// The (row, head) pairs that read one KV head of one sequence are columns of a
-// tile of 8 NT; a page's 16 tokens are the rows of m16n8k16 products:
+// The (row, head) pairs that read one KV head of one sequence are columns; a
+// page's 16 tokens are the rows of m16n8k16 products:
 //   S^T [16 tokens x 8] = K Q^T,  O^T [HD x 8] += V^T P^T.
 // The cache words are laid out as the products' A operands, so a code goes
 // from shared memory to the tensor core through registers only:
@@ -10,18 +10,30 @@
 //      high nibbles' k-steps.  A block's 32 dims are two k-steps, and
 //      s = sum_b d_b (acc_b - z_b sum_b(q)) puts step and zero point in after
 //      the integer product, in fp32.
-//   V: (q - z) d is formed in registers, exact in fp16 (the format's steps have
-//      7 significant bits).
+//   V: a nibble in place times D plus Z is (q - z) d 2^(e - 24) in one fused
+//      multiply-add, with D = d 2^e (high nibbles: d 2^(e - 4)) and Z = -z d
+//      2^(e - 24).  e is the warp's: the largest d so far becomes 2^13 to 2^16,
+//      and O is rescaled when a larger one comes.  All of it is exact for d
+//      down to 2^-7 of that, and to 2^-25 of the largest product below.
 // Q (scaled by a power of two to below 2^14) and P (2^7 times the softmax
-// weight) are split into an fp16 high part and an fp16 residual, multiplied
-// one after the other: results keep fp32 accuracy.  Softmax in base 2 with a
-// running reference; it moves (and O is rescaled) only when a score exceeds it
-// by more than 8, so that weights stay within fp16.
+// weight) are an fp16 high part plus an fp16 residual: results keep fp32
+// accuracy.  Up to four columns, the two parts are two columns of one product
+// (no padding, half the products); beyond, two products into one accumulator,
+// the residuals' first in K Q^T.  Softmax in base 2 with a running reference;
+// it moves (and O is rescaled) only when a score exceeds it by more than 8, so
+// that weights stay within fp16.
 //
-// kNarrowWarps warps take the split's pages in turn.  Each has its own ring of
-// page buffers, filled by one bulk copy per page (a page's 18 HD bytes of one
-// KV head are contiguous).  The warps' states merge in shared memory, splits of
-// the context through the workspace in the last CTA of a tile, in split order.
+// The pages of all tiles (entry, column tile, KV head) in a row are dealt out
+// in equal runs to as many CTAs as the GPU holds at once, whatever the
+// sequences' lengths; a CTA walks the parts of tiles that its run covers (one
+// part where there are twice as many CTAs as tiles: every tile then starts a
+// run).  Its
+// kNarrowWarps warps take a part's pages in turn, two at a time where registers
+// allow (one softmax step and twice the independent products).  Each has its
+// own ring of page buffers, filled by bulk copies (a page's 18 HD bytes of one
+// KV head are contiguous); the next part's first copies are under way while a
+// part is written.  The warps' states merge in shared memory, the parts of a
+// tile through the workspace in a second kernel, in page order.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -36,39 +48,17 @@
 namespace axq8 {
 
 constexpr int kNarrowWarps = 4;
-constexpr int kNarrowBufs = 4;        // pages in flight per warp
-constexpr int kNarrowMinPages = 8;    // pages of a split at least
-constexpr int kNarrowMaxSplits = 128;
+constexpr int kNarrowPages = 4;       // page buffers of a warp
+constexpr int kNarrowMinPages = 24;   // pages of a run at least
+constexpr int kNarrowMaxParts = 96;   // parts of a tile at most (one CTA joins them)
+constexpr int kJoinThreads = 256;
+constexpr int kNarrowTileCost = 10;   // what a tile costs beside its pages, in pages
+constexpr int kNarrowKept = 128;      // entries kept in shared memory (else read again)
 
 struct Kv4Pages {
     uint8_t* pages;
     const int* table;
     int n_seqs, max_blocks, n_pages, n_kv;
-};
-
-struct NarrowArgs {
-    Kv4Pages c;
-    const float* q;
-    int64_t ldq;
-    int n_rows, max_rows, n_heads, G, nsplit;
-    const int* q_seq;
-    const int* q_start;   // null: one row per entry
-    const int* q_pos;
-    float scale;          // softmax scale times log2(e)
-    float* out;
-    float* part;          // [tile][split][8 NT][HD], then [tile][split][8 NT][2]
-    int* counters;        // one per tile
-    int* status;
-};
-
-template <int HD, int NT>
-struct NarrowCfg {
-    static constexpr int COLS = 8 * NT;
-    static constexpr int PITCH = HD + 4;   // merge rows, conflict-free
-    static constexpr size_t RING = (size_t)kNarrowWarps * kNarrowBufs * Kv4<HD>::BYTES;
-    static constexpr size_t MERGE = (size_t)kNarrowWarps * COLS * (PITCH + 2) * 4;
-    static constexpr size_t BAR = RING > MERGE ? RING : MERGE;
-    static constexpr size_t SMEM = BAR + kNarrowWarps * kNarrowBufs * 8;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -104,6 +94,34 @@ __device__ __forceinline__ uint32_t hfma2u(uint32_t a, uint32_t b, uint32_t c) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Bounded wait for a copy: the hardware suspends the warp for up to 20 us at a
+// time, a second in all.
+__device__ __forceinline__ bool copy_wait(uint64_t* bar, uint32_t parity) {
+    for (int i = 0; i < 50000; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+// c = a b, the first product of a sum.
+__device__ __forceinline__ void mma_f16_16816_first(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// 2^k as fp16 in both halves, -14 <= k <= 15.
+__device__ __forceinline__ uint32_t f16_pow2(int k) { return (uint32_t)(k + 15) * 0x04000400u; }
+
 // N 32-bit words from shared memory, as wide as N allows (aligned to 4 N bytes, 16 at most).
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[N], const uint8_t* p) {
@@ -131,91 +149,354 @@ struct Scales {
     }
 };
 
-template <int HD, int NT>
-__global__ void __launch_bounds__(kNarrowWarps * 32) kv4_attn_narrow_kernel(const NarrowArgs a) {
+struct NarrowArgs {
+    Kv4Pages c;
+    const float* q;
+    int64_t ldq;
+    int n_rows, n_entries, max_rows, n_heads, G;
+    int aligned;          // every tile starts a run
+    const int* q_seq;
+    const int* q_start;   // null: one row per entry
+    const int* q_pos;
+    float scale;          // softmax scale times log2(e)
+    float* out;
+    struct NarrowPart* split;   // [CTA]: the tile whose first part is this CTA's, if it has more
+    float* part;          // [CTA][2][COLS][HD], then [CTA][2][COLS][2]
+    int* status;
+};
+
+// Entry i of the request: its rows, sequence, and the pages of its tiles.
+struct NarrowEntry {
+    int r0, T, seq, pos0, ctx, nblk, segs;   // segs: tiles of nblk pages each
+};
+__device__ __forceinline__ NarrowEntry narrow_entry(const NarrowArgs& a, int i, int cols, bool report) {
+    NarrowEntry e;
+    const int room = a.c.max_blocks * kKv4Tokens;
+    e.r0 = i;
+    e.T = 1;
+    bool ok = true;
+    if (a.q_start) {
+        e.r0 = a.q_start[i];
+        e.T = a.q_start[i + 1] - e.r0;
+        ok = e.T <= 0 || (e.r0 >= 0 && e.r0 <= a.n_rows - e.T && e.T <= a.max_rows);
+        if (!ok) e.T = 0;
+    }
+    e.seq = a.q_seq ? a.q_seq[i] : i;
+    e.pos0 = min(a.q_pos[i], room);
+    const bool seq_ok = e.seq >= 0 && e.seq < a.c.n_seqs;
+    if (report && (!ok || (e.T > 0 && (!seq_ok || e.pos0 + e.T > room))))
+        record_status(a.status, AXQ8_ERR_INVALID);
+    e.ctx = seq_ok ? max(0, min(e.pos0 + e.T, room)) : 0;
+    if (!seq_ok) e.seq = 0;
+    // no token at all: one page that nothing sees, so that the zeros are written
+    e.nblk = max(1, (e.ctx + kKv4Tokens - 1) / kKv4Tokens);
+    e.segs = e.T > 0 ? (e.T * a.G + cols - 1) / cols * a.c.n_kv : 0;
+    return e;
+}
+
+// A part of a tile: what a CTA works on at a time.
+struct NarrowPart {
+    int r0, cols, seq, pos0, ctx;   // the entry's first row, columns, sequence, first position, tokens
+    int kvh, col0;                  // the tile
+    int b0, b1;                     // pages of the part
+    int c0, c1;                     // CTAs with parts of the tile; b0 == b1: no part
+};
+
+// A CTA's run: units [p, end) of all tiles' units in a row.  A tile's units are
+// `before` of no page (what a tile costs beside its pages), its pages, and in
+// the aligned case more of no page up to a multiple of the run.
+struct NarrowRun {
+    int p, end, run, before;
+    int entry, first;   // the entry at p, and its first unit
+    __device__ __forceinline__ int units(const NarrowArgs& a, int nblk) const {
+        return a.aligned ? (nblk + run - 1) / run * run : nblk + before;
+    }
+};
+
+// The part at r.p, and r.p past it (one thread); d.b0 == d.b1: none is left.
+template <int COLS>
+__device__ __noinline__ void narrow_next_part(const NarrowArgs& a, const NarrowEntry* kept, NarrowRun& r,
+                                              NarrowPart& d) {
+    int p = r.p, first = r.first, i = r.entry;
+    d.b0 = d.b1 = 0;
+    while (p < r.end) {
+        const NarrowEntry e = kept ? kept[i] : narrow_entry(a, i, COLS, false);
+        const int units = r.units(a, e.nblk);
+        if (p >= first + units * e.segs) {
+            first += units * e.segs;
+            i++;
+            continue;
+        }
+        const int seg = (p - first) / units;
+        const int tile = first + seg * units + r.before;   // its first page
+        const int stop = min(r.end, first + (seg + 1) * units), last = min(stop, tile + e.nblk);
+        if (last > max(tile, p)) {
+            d.r0 = e.r0;
+            d.cols = e.T * a.G;
+            d.seq = e.seq;
+            d.pos0 = e.pos0;
+            d.ctx = e.ctx;
+            d.kvh = seg % a.c.n_kv;
+            d.col0 = seg / a.c.n_kv * COLS;
+            d.b0 = max(0, p - tile);
+            d.b1 = last - tile;
+            d.c0 = tile / r.run;
+            d.c1 = (tile + e.nblk - 1) / r.run;
+        }
+        p = stop;
+        if (d.b1 > 0) break;
+    }
+    r.p = p;
+    r.first = first;
+    r.entry = i;
+}
+
+__device__ __forceinline__ void narrow_write(const NarrowArgs& a, const NarrowPart& d, int HD, int col, int dim,
+                                             float4 v, float sum) {
+    const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;   // nothing seen: zeros
+    const int c = d.col0 + col, j = c / a.G;
+    *reinterpret_cast<float4*>(a.out + (int64_t)(d.r0 + j) * a.n_heads * HD +
+                               (int64_t)(d.kvh * a.G + c - j * a.G) * HD + dim) =
+        make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+}
+
+// COLS columns of a tile: 4 (both parts of Q and P in one n-tile), 8 or 16.
+template <int HD, int COLS_>
+struct NarrowCfg {
+    static constexpr int COLS = COLS_;
+    static constexpr bool PACK = COLS == 4;
+    static constexpr int NT = COLS <= 8 ? 1 : 2;        // n-tiles of 8
+    static constexpr int PP = COLS <= 8 ? 2 : 1;        // pages of a step
+    static constexpr int NBUF = kNarrowPages / PP;      // steps in flight
+    static constexpr int PITCH = HD + 4;                // merge rows, conflict-free
+    static constexpr size_t RING = (size_t)kNarrowWarps * kNarrowPages * Kv4<HD>::BYTES;
+    static constexpr size_t MERGE = RING;               // the warps' states
+    static constexpr size_t VSC = MERGE + (size_t)kNarrowWarps * COLS * (PITCH + 2) * 4;   // V factors
+    static constexpr size_t VSC_PAGE = 4 * 2 * Kv4<HD>::NB * 8;  // [t][block][u] {D, Z}
+    static constexpr size_t QBUF = VSC + kNarrowWarps * PP * VSC_PAGE;   // Q of this and the next part
+    static constexpr size_t KEPT = QBUF + 2 * COLS * HD * 4;
+    static constexpr size_t BAR = KEPT + kNarrowKept * sizeof(NarrowEntry);
+    static constexpr size_t SMEM = BAR + kNarrowWarps * NBUF * 8;
+    static constexpr int JOIN_ITEMS = COLS * HD / 4 < 64 ? COLS * HD / 4 : 64;   // 4 dims of a column each
+    static constexpr int CTAS = COLS == 4 ? 4 : COLS == 8 ? 3 : 2;   // resident per SM
+};
+
+// The parts of the tile that begins in run blockIdx.x, joined in page order: the
+// second slot of CTA c0, then the first slots of c0 + 1 .. c1.  Groups of threads
+// take every S-th part of a column's 4 dims each; group states join the same way.
+template <int HD, int COLS>
+__global__ void __launch_bounds__(kJoinThreads) kv4_attn_join_kernel(const __grid_constant__ NarrowArgs a) {
+    constexpr int PER = NarrowCfg<HD, COLS>::JOIN_ITEMS, S = kJoinThreads / PER;
+    __shared__ float4 acc_s[S][PER];
+    __shared__ float2 ml_s[S][PER];
+    pdl_wait();
+    const NarrowPart& d = a.split[blockIdx.x];
+    const int c0 = d.c0, c1 = d.c1;
+    if (c1 <= c0) return;
+    const float* pml = a.part + (int64_t)gridDim.x * 2 * COLS * HD;
+    const int live = min(COLS, d.cols - d.col0), group = threadIdx.x / PER, item = threadIdx.x % PER;
+    const int idx = blockIdx.y * PER + item, col = idx / (HD / 4), dim = idx % (HD / 4) * 4;
+    if (blockIdx.y * PER >= live * (HD / 4)) return;
+    float mx = -CUDART_INF_F, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](float2 ml, float4 x) {
+        if (ml.x == -CUDART_INF_F) return;
+        const float m = fmaxf(mx, ml.x), f = ex2(mx - m), h = ex2(ml.x - m);
+        mx = m;
+        v.x = fmaf(v.x, f, x.x * h);
+        v.y = fmaf(v.y, f, x.y * h);
+        v.z = fmaf(v.z, f, x.z * h);
+        v.w = fmaf(v.w, f, x.w * h);
+        sum = fmaf(sum, f, ml.y * h);
+    };
+    for (int k0 = c0 + group; k0 <= c1; k0 += 8 * S) {
+        float2 ml[8];
+        float4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const int k = k0 + u * S;
+            ml[u] = make_float2(-CUDART_INF_F, 0.0f);
+            if (k <= c1) {
+                const int64_t at = ((int64_t)k * 2 + (k == c0)) * COLS + col;
+                ml[u] = ld_cg2(pml + at * 2);
+                x[u] = ld_cg4(a.part + at * HD + dim);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++) add(ml[u], x[u]);
+    }
+    acc_s[group][item] = v;
+    ml_s[group][item] = make_float2(mx, sum);
+    __syncthreads();
+    if (group == 0 && idx < live * (HD / 4)) {
+#pragma unroll
+        for (int k = 1; k < S; k++) add(ml_s[k][item], acc_s[k][item]);
+        narrow_write(a, d, HD, col, dim, v, sum);
+    }
+}
+
+template <int HD, int COLS>
+__global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
+    kv4_attn_narrow_kernel(const __grid_constant__ NarrowArgs a) {
     using F = Kv4<HD>;
-    using C = NarrowCfg<HD, NT>;
-    constexpr int NB = F::NB, MT = F::TILES, W = kNarrowWarps, NBUF = kNarrowBufs;
+    using C = NarrowCfg<HD, COLS>;
+    constexpr int NB = F::NB, MT = F::TILES, W = kNarrowWarps, NBUF = C::NBUF, NT = C::NT, PP = C::PP;
+    constexpr bool PACK = C::PACK;
+    constexpr int STEP = PP * F::BYTES;
     extern __shared__ __align__(16) uint8_t nar_sm[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int kvh = blockIdx.x % a.c.n_kv, ct = blockIdx.x / a.c.n_kv;
-    const int i = blockIdx.y, sp = blockIdx.z;
-    const int tile = (i * (gridDim.x / a.c.n_kv) + ct) * a.c.n_kv + kvh;
-
-    // the entry's rows, sequence and positions
-    int r0 = i, T = 1;
-    if (a.q_start) {
-        r0 = __ldg(a.q_start + i);
-        T = __ldg(a.q_start + i + 1) - r0;
-        if (T <= 0) return;
-        if (r0 < 0 || r0 > a.n_rows - T || T > a.max_rows) {
-            if (threadIdx.x == 0) record_status(a.status, AXQ8_ERR_INVALID);
-            return;
-        }
-    }
-    const int cols = T * a.G, col0 = ct * C::COLS;
-    if (col0 >= cols) return;
-    const int seq = a.q_seq ? __ldg(a.q_seq + i) : i;
+    // this lane's column of Q^T operands, and the first of its two in the accumulators
+    const int gq = PACK ? g & 3 : g, tq = PACK ? 2 * (t & 1) : 2 * t;
     const int room = a.c.max_blocks * kKv4Tokens;
-    const bool seq_ok = seq >= 0 && seq < a.c.n_seqs;
-    const int pos0 = min(__ldg(a.q_pos + i), room);
-    if ((!seq_ok || pos0 + T > room) && threadIdx.x == 0) record_status(a.status, AXQ8_ERR_INVALID);
-    const int jmax = min(T - 1, (col0 + C::COLS - 1) / a.G);
-    const int ctx = seq_ok ? max(0, min(pos0 + jmax + 1, room)) : 0;
-    const int nblk = (ctx + kKv4Tokens - 1) / kKv4Tokens;
-    const int pps = max(kNarrowMinPages, (nblk + a.nsplit - 1) / a.nsplit);
-    const int ns = max(1, (nblk + pps - 1) / pps);
-    if (sp >= ns) return;
-    const int b0 = sp * pps, b1 = min(nblk, b0 + pps);
-
-    // page ring of this warp
-    uint8_t* ring = nar_sm + (size_t)warp * NBUF * F::BYTES;
+    if (threadIdx.x == 0) {   // no tile of several parts begins here, as yet
+        a.split[blockIdx.x].c0 = a.split[blockIdx.x].c1 = 0;
+        pdl_launch_dependents();
+    }
+    uint8_t* ring = nar_sm + (size_t)warp * NBUF * STEP;
     uint64_t* full = reinterpret_cast<uint64_t*>(nar_sm + C::BAR) + warp * NBUF;
+    uint8_t* vsc = nar_sm + C::VSC + warp * (PP * C::VSC_PAGE);
+    float* acc_s = reinterpret_cast<float*>(nar_sm + C::MERGE);         // [W][COLS][PITCH]
+    float* ml_s = acc_s + (size_t)W * COLS * C::PITCH;                  // [W][COLS][2]
     if (lane == 0) {
         for (int s = 0; s < NBUF; s++) mbar_init(full + s, 1);
         fence_mbar_init();
     }
-    __syncwarp();
-    const int npw = b1 > b0 + warp ? (b1 - b0 - warp + W - 1) / W : 0;
-    const int* row_table = a.c.table + (int64_t)(seq_ok ? seq : 0) * a.c.max_blocks;
-    int ids = -1;            // lane l: the id of this warp's page 32 (n / 32) + l
-    uint32_t bad = 0;        // bit s: the page of buffer s is outside the pool
-    auto issue = [&](int n) {
-        if ((n & 31) == 0) {
-            const int blk = b0 + warp + (n + lane) * W;
-            ids = blk < b1 ? __ldg(row_table + blk) : 0;
-        }
-        const int page = __shfl_sync(0xffffffffu, ids, n & 31), s = n % NBUF;
-        const bool ok = page >= 0 && page < a.c.n_pages;
-        bad = (bad & ~(1u << s)) | ((ok ? 0u : 1u) << s);
-        if (lane == 0) {
-            if (ok) {
-                mbar_arrive_expect_tx(full + s, F::BYTES);
-                bulk_g2s(ring + s * F::BYTES, a.c.pages + ((int64_t)page * a.c.n_kv + kvh) * F::BYTES,
-                         F::BYTES, full + s);
-            } else {
-                record_status(a.status, AXQ8_ERR_INVALID);
-                mbar_arrive(full + s);
+
+    float* qbuf = reinterpret_cast<float*>(nar_sm + C::QBUF);          // [2][COLS][HD]
+    NarrowEntry* kept = a.n_entries <= kNarrowKept ? reinterpret_cast<NarrowEntry*>(nar_sm + C::KEPT) : nullptr;
+    __shared__ int scan_sm[2][2][W];
+    __shared__ NarrowRun run_s;
+    __shared__ NarrowPart parts[3];     // the last, this and the next one
+    {
+        const int per = (a.n_entries + W * 32 - 1) / (W * 32), i0 = threadIdx.x * per;
+        const int before = a.aligned ? 0 : kNarrowTileCost;
+        // pass 0: all units without alignment give the run; pass 1: the units of
+        // the threads up to this one
+        int run = 1, total = 0, longest = 1, mine = 0, upto = 0;
+#pragma unroll 1
+        for (int pass = 0; pass < 2; pass++) {
+            mine = 0;
+            for (int i = i0; i < min(i0 + per, a.n_entries); i++) {
+                const NarrowEntry e = kept && pass ? kept[i] : narrow_entry(a, i, COLS, blockIdx.x == 0 && !pass);
+                if (kept && !pass) kept[i] = e;
+                const int n = e.nblk + before;
+                mine += (a.aligned ? (n + run - 1) / run * run : n) * e.segs;
+                longest = max(longest, n);
             }
+            upto = mine;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, s);
+                if (lane >= s) upto += v;
+            }
+            longest = __reduce_max_sync(0xffffffffu, longest);
+            if (lane == 31) {
+                scan_sm[pass][0][warp] = upto;
+                scan_sm[pass][1][warp] = longest;
+            }
+            __syncthreads();
+            upto -= mine;
+            total = 0;
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                if (w < warp) upto += scan_sm[pass][0][w];
+                total += scan_sm[pass][0][w];
+                longest = max(longest, scan_sm[pass][1][w]);
+            }
+            if (pass) break;
+            // aligned: at most `tiles` more runs than the units fill
+            const int ctas = gridDim.x - a.aligned;
+            run = max(max(kNarrowMinPages, (total + ctas - 1) / ctas), (longest + kNarrowMaxParts - 1) / kNarrowMaxParts);
+            if (!a.aligned) break;
+        }
+        const int p = blockIdx.x * run;
+        if (p >= total) return;
+        if (p >= upto && p < upto + mine) {   // one thread: the entry that holds unit p
+            NarrowRun r;
+            r.p = p;
+            r.end = min(total, p + run);
+            r.run = run;
+            r.before = before;
+            r.first = upto;
+            r.entry = i0;
+            run_s = r;
+            narrow_next_part<COLS>(a, kept, run_s, parts[0]);
+        }
+        __syncthreads();
+    }
+    if (parts[0].b1 <= parts[0].b0) return;   // no page of a tile in the run
+    // the part's Q rows to buffer `to`, zeros behind its columns
+    auto fetch_q = [&](const NarrowPart& d, int to) {
+        for (int idx = threadIdx.x; idx < COLS * (HD / 4); idx += W * 32) {
+            const int col = idx / (HD / 4), c = d.col0 + col, j = c / a.G;
+            const bool ok = c < d.cols;
+            const float* src = a.q + (ok ? (int64_t)(d.r0 + j) * a.ldq + (int64_t)(d.kvh * a.G + c - j * a.G) * HD +
+                                               idx % (HD / 4) * 4 : 0);
+            cp_async16_zfill(qbuf + to * COLS * HD + idx * 4, src, ok);
+        }
+        cp_async_commit();
+    };
+    fetch_q(parts[0], 0);
+
+    int ids = -1;            // lane l: the id of the l-th page from step n / (32 / PP) * (32 / PP) on
+    uint32_t bad = 0;        // bit PP s + k: page k of buffer s is none
+    unsigned used = 0;       // steps of this warp so far, over all parts
+    bool lost = false;       // a copy never came: compute nothing more
+    auto steps_of = [&](const NarrowPart& d) {
+        const int steps = (d.b1 - d.b0 + PP - 1) / PP;
+        return steps > warp && !lost ? (steps - warp + W - 1) / W : 0;
+    };
+    // step n of this warp in part d: pages b0 + (n W + warp) PP + 0 .. PP - 1
+    auto issue = [&](const NarrowPart& d, int n) {
+        if (n % (32 / PP) == 0) {
+            const int blk = d.b0 + ((n + lane / PP) * W + warp) * PP + lane % PP;
+            const bool live = blk < d.b1 && blk * kKv4Tokens < d.ctx;
+            ids = live ? __ldg(a.c.table + (int64_t)d.seq * a.c.max_blocks + blk) : -1;
+            if (live && (unsigned)ids >= (unsigned)a.c.n_pages) record_status(a.status, AXQ8_ERR_INVALID);
+        }
+        const int s = (used + n) % NBUF;
+        int page[PP], bytes = 0;
+#pragma unroll
+        for (int k = 0; k < PP; k++) {
+            page[k] = __shfl_sync(0xffffffffu, ids, (n * PP + k) & 31);
+            const bool ok = (unsigned)page[k] < (unsigned)a.c.n_pages;
+            bad = (bad & ~(1u << (PP * s + k))) | ((ok ? 0u : 1u) << (PP * s + k));
+            if (!ok) page[k] = -1;
+            else bytes += F::BYTES;
+        }
+        if (lane == 0) {
+            const uint8_t* src = a.c.pages + d.kvh * F::BYTES;
+            const int pitch = a.c.n_kv * F::BYTES;
+            mbar_arrive_expect_tx(full + s, bytes);
+#pragma unroll
+            for (int k = 0; k < PP; k++)
+                if (page[k] >= 0)
+                    bulk_g2s(ring + s * STEP + k * F::BYTES, src + (int64_t)page[k] * pitch, F::BYTES, full + s);
         }
     };
-    for (int n = 0; n < min(npw, NBUF); n++) issue(n);
+    for (int n = 0; n < min(steps_of(parts[0]), NBUF); n++) issue(parts[0], n);
+    if (threadIdx.x == 0) narrow_next_part<COLS>(a, kept, run_s, parts[1]);
+    cp_async_wait_all();
+    __syncthreads();   // Q is there, and the second part
 
-    // Q^T operands (column g), their block sums and scales (columns 2t, 2t + 1)
-    uint32_t qh[NT][NB][4], ql[NT][NB][4];
+  for (int which = 0, qb = 0;; which = which == 2 ? 0 : which + 1, qb ^= 1) {
+    const NarrowPart& part = parts[which];
+    const NarrowPart& next = parts[which == 2 ? 0 : which + 1];
+    const int part_steps = steps_of(part), part_b0 = part.b0, ctx = part.ctx;
+
+    // Q^T operands (column gq), their block sums and scales (columns tq, tq + 1)
+    uint32_t qh[NT][NB][4], ql[PACK ? 1 : NT][PACK ? 1 : NB][4];
     float qs[NT][2][NB], mul[NT][2];
     int lim[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int col = col0 + 8 * n + g, j = col / a.G;
         float x[NB][8], mx = 0.0f;
-        const float* qp = a.q + (int64_t)(r0 + j) * a.ldq + (int64_t)(kvh * a.G + col - j * a.G) * HD;
+        const float* qp = qbuf + (qb * COLS + 8 * n + gq) * HD;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (col < cols) v = __ldg(reinterpret_cast<const float4*>(qp + 32 * b + 8 * t + e));
+                const float4 v = *reinterpret_cast<const float4*>(qp + 32 * b + 8 * t + e);
                 x[b][e] = v.x;
                 x[b][e + 1] = v.y;
                 x[b][e + 2] = v.z;
@@ -231,16 +512,24 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) kv4_attn_narrow_kernel(cons
         float sum[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
+            constexpr int first[4] = {0, 2, 1, 3};   // elements of operand register k: (first, first + 4)
             sum[b] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[b][e] *= up;
-                sum[b] += x[b][e];
+            for (int k = 0; k < 4; k++) {
+                const float f = k < 2 ? 1.0f : 0.0625f;
+                const float x0 = x[b][first[k]] * up, x1 = x[b][first[k] + 4] * up;
+                uint32_t hi, lo;
+                split2(x0 * f, x1 * f, hi, lo);
+                if (PACK) {   // columns 4 .. 7 are the residuals of columns 0 .. 3
+                    qh[n][b][k] = g < 4 ? hi : lo;
+                    const float2 v = f16_pair(qh[n][b][k]);
+                    sum[b] += (v.x + v.y) * (k < 2 ? 1.0f : 16.0f);
+                } else {
+                    qh[n][b][k] = hi;
+                    ql[n][b][k] = lo;
+                    sum[b] += x0 + x1;
+                }
             }
-            split2(x[b][0], x[b][4], qh[n][b][0], ql[n][b][0]);
-            split2(x[b][2], x[b][6], qh[n][b][1], ql[n][b][1]);
-            split2(x[b][1] * 0.0625f, x[b][5] * 0.0625f, qh[n][b][2], ql[n][b][2]);
-            split2(x[b][3] * 0.0625f, x[b][7] * 0.0625f, qh[n][b][3], ql[n][b][3]);
             sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 1);
             sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 2);
         }
@@ -250,8 +539,8 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) kv4_attn_narrow_kernel(cons
 #pragma unroll
             for (int b = 0; b < NB; b++) qs[n][hh][b] = __shfl_sync(0xffffffffu, sum[b], src);
             mul[n][hh] = __shfl_sync(0xffffffffu, down, src);
-            const int cc = col0 + 8 * n + 2 * t + hh;
-            lim[n][hh] = cc < cols ? min(pos0 + cc / a.G + 1, room) : 0;
+            const int cc = part.col0 + 8 * n + tq + hh;
+            lim[n][hh] = cc < part.cols ? min(part.pos0 + cc / a.G + 1, room) : 0;
         }
     }
     int low = ctx;   // tokens that every live column sees
@@ -259,9 +548,12 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) kv4_attn_narrow_kernel(cons
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int hh = 0; hh < 2; hh++)
-            if (col0 + 8 * n + 2 * t + hh < cols) low = min(low, lim[n][hh]);
+            if (part.col0 + 8 * n + tq + hh < part.cols) low = min(low, lim[n][hh]);
     low = __reduce_min_sync(0xffffffffu, low);
 
+    const float rest = t < 2 ? 0.0f : -1.0f;
+    int dexp = 0;           // e: O holds the sum times 2^(e - 24)
+    uint32_t dtop = 0;      // bits of the d from which e has to fall
     float o[NT][MT][4], base[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -271,170 +563,248 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) kv4_attn_narrow_kernel(cons
         for (int m = 0; m < MT; m++) o[n][m][0] = o[n][m][1] = o[n][m][2] = o[n][m][3] = 0.0f;
     }
 
-    for (int it = 0; it < npw; it++) {
-        const int s = it % NBUF;
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(full + s, (it / NBUF) & 1, a.status,
-                                                       AXQ8_ERR_WAIT_TIMEOUT))) {
-            // no copy may still be landing when the CTA reuses its shared memory
-            for (int n = it + 1; n < min(npw, it + NBUF); n++)
-                mbar_wait_bounded(full + n % NBUF, (n / NBUF) & 1, a.status, AXQ8_ERR_WAIT_TIMEOUT);
+    for (int it = 0; it < part_steps; it++) {
+        const int s = (used + it) % NBUF;
+        if (!__all_sync(0xffffffffu, copy_wait(full + s, ((used + it) / NBUF) & 1))) {
+            // a copy was lost: no other may still be landing when the CTA ends
+            if (lane == 0) record_status(a.status, AXQ8_ERR_WAIT_TIMEOUT);
+            for (unsigned n = used + it + 1; n < used + min(part_steps, it + NBUF); n++)
+                copy_wait(full + n % NBUF, (n / NBUF) & 1);
+            lost = true;   // and none is started
             break;
         }
-        const uint8_t* pg = ring + s * F::BYTES;
-        const int tok0 = (b0 + warp + it * W) * kKv4Tokens;
-        if (!((bad >> s) & 1)) {
-            // scores: tokens g (sc[..][0], [1]) and g + 8 ([2], [3]), columns 2t, 2t + 1
-            float sc[NT][4];
+        const uint8_t* buf = ring + s * STEP;
+        int tok0[PP];   // first token of a page; no page: one that nothing sees
 #pragma unroll
-            for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
-            {
-                uint32_t w0[NB], w1[NB];
-                lds_words<NB>(w0, pg + g * (HD / 2) + t * (HD / 8));
-                lds_words<NB>(w1, pg + (g + 8) * (HD / 2) + t * (HD / 8));
-                Scales<NB> s0, s1;
-                s0.load(pg + F::KS, g);
-                s1.load(pg + F::KS, g + 8);
+        for (int p = 0; p < PP; p++)
+            tok0[p] = (bad >> (PP * s + p)) & 1 ? 0x40000000
+                                                : (part_b0 + (it * W + warp) * PP + p) * kKv4Tokens;
+        // V factors: lane (g, t) makes those of block b = g % NB, tokens 2t + 8u, 2t + 1 + 8u
+        uint32_t dz[PP][2], dmax = 0;
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const uint32_t u0 = w0[b] >> 8, u1 = w1[b] >> 8;
-                    const uint32_t lowa[4] = {w0[b] & 0x000f000fu, w1[b] & 0x000f000fu,
-                                              u0 & 0x000f000fu, u1 & 0x000f000fu};
-                    const uint32_t higha[4] = {w0[b] & 0x00f000f0u, w1[b] & 0x00f000f0u,
-                                               u0 & 0x00f000f0u, u1 & 0x00f000f0u};
-                    const float2 d0p = f16_pair(s0.word(b) & 0x7ff07ff0u), z0p = f16_pair(s0.word(b) & 0x000f000fu);
-                    const float2 d1p = f16_pair(s1.word(b) & 0x7ff07ff0u), z1p = f16_pair(s1.word(b) & 0x000f000fu);
-                    const float d0 = b & 1 ? d0p.y : d0p.x, z0 = b & 1 ? z0p.y : z0p.x;
-                    const float d1 = b & 1 ? d1p.y : d1p.x, z1 = b & 1 ? z1p.y : z1p.x;
+        for (int p = 0; p < PP; p++) {
+            const uint8_t* vs = buf + p * F::BYTES + F::VS;
+            const int u = g / NB, r = 2 * t + 8 * (u & 1), b = g % NB;
+            uint32_t wa = *reinterpret_cast<const uint16_t*>(vs + F::scale(r, b));
+            uint32_t wb = *reinterpret_cast<const uint16_t*>(vs + F::scale(r + 1, b));
+            if (tok0[p] + kKv4Tokens > ctx) {   // slots behind the last token: any bits
+                if (tok0[p] + r >= ctx) wa = 0;
+                if (tok0[p] + r + 1 >= ctx) wb = 0;
+            }
+            dmax = max(dmax, max(wa, wb));
+            const uint32_t w = __byte_perm(wa, wb, 0x5410);
+            dz[p][0] = w & 0x7ff07ff0u;
+            dz[p][1] = w & 0x000f000fu;
+        }
+        dmax = __reduce_max_sync(0xffffffffu, dmax);   // the largest d, and some zero point
+        if (dmax >= dtop) {                            // beyond 2^16 / 2^e
+            const int ne = 28 - (int)(dmax >> 10);
+            const float f = __uint_as_float((uint32_t)(127 + ne - dexp) << 23);
+            dexp = ne;
+            dtop = (uint32_t)(31 - ne) << 10;
+            if (it) {
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int k = 0; k < MT; k++) {
+                        o[n][k][0] *= f;
+                        o[n][k][1] *= f;
+                        o[n][k][2] *= f;
+                        o[n][k][3] *= f;
+                    }
+            }
+        }
+        {
+            const uint32_t up1 = f16_pow2(dexp / 2), up2 = f16_pow2(dexp - dexp / 2);
+#pragma unroll
+            for (int p = 0; p < PP; p++) {
+                const uint32_t D = hmul2u(hmul2u(dz[p][0], up1), up2);
+                const uint32_t Z = hmul2u(dz[p][1], D) ^ 0x80008000u;
+                if (g < 2 * NB)
+                    *reinterpret_cast<uint2*>(vsc + p * C::VSC_PAGE + ((t * NB + g % NB) * 2 + g / NB) * 8) =
+                        make_uint2(D, Z);
+            }
+        }
+        // scores: tokens g (sc[..][0], [1]) and g + 8 ([2], [3]), columns tq, tq + 1
+        float sc[PP][NT][4];
+#pragma unroll
+        for (int p = 0; p < PP; p++) {
+            const uint8_t* pg = buf + p * F::BYTES;
+#pragma unroll
+            for (int n = 0; n < NT; n++) sc[p][n][0] = sc[p][n][1] = sc[p][n][2] = sc[p][n][3] = 0.0f;
+            uint32_t w0[NB], w1[NB];
+            lds_words<NB>(w0, pg + g * (HD / 2) + t * (HD / 8));
+            lds_words<NB>(w1, pg + (g + 8) * (HD / 2) + t * (HD / 8));
+            Scales<NB> s0, s1;
+            s0.load(pg + F::KS, g);
+            s1.load(pg + F::KS, g + 8);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const uint32_t u0 = w0[b] >> 8, u1 = w1[b] >> 8;
+                const uint32_t lowa[4] = {w0[b] & 0x000f000fu, w1[b] & 0x000f000fu,
+                                          u0 & 0x000f000fu, u1 & 0x000f000fu};
+                const uint32_t higha[4] = {w0[b] & 0x00f000f0u, w1[b] & 0x00f000f0u,
+                                           u0 & 0x00f000f0u, u1 & 0x00f000f0u};
+                const float2 d0p = f16_pair(s0.word(b) & 0x7ff07ff0u), z0p = f16_pair(s0.word(b) & 0x000f000fu);
+                const float2 d1p = f16_pair(s1.word(b) & 0x7ff07ff0u), z1p = f16_pair(s1.word(b) & 0x000f000fu);
+                const float d0 = b & 1 ? d0p.y : d0p.x, z0 = b & 1 ? z0p.y : z0p.x;
+                const float d1 = b & 1 ? d1p.y : d1p.x, z1 = b & 1 ? z1p.y : z1p.x;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float c[4];
+                    if constexpr (PACK) {
+                        mma_f16_16816_first(c, lowa, qh[n][b][0], qh[n][b][1]);
+                    } else {
                         // residuals first: the product truncates each sum to the
                         // accumulator's 24 bits, which costs less while it is small
-                        mma_f16_16816(c, lowa, ql[n][b][0], ql[n][b][1]);
+                        mma_f16_16816_first(c, lowa, ql[n][b][0], ql[n][b][1]);
                         mma_f16_16816(c, higha, ql[n][b][2], ql[n][b][3]);
                         mma_f16_16816(c, lowa, qh[n][b][0], qh[n][b][1]);
-                        mma_f16_16816(c, higha, qh[n][b][2], qh[n][b][3]);
-#pragma unroll
-                        for (int hh = 0; hh < 2; hh++) {
-                            sc[n][hh] = fmaf(d0, fmaf(-z0, qs[n][hh][b], c[hh]), sc[n][hh]);
-                            sc[n][2 + hh] = fmaf(d1, fmaf(-z1, qs[n][hh][b], c[2 + hh]), sc[n][2 + hh]);
-                        }
                     }
-                }
-            }
-            bool over = false;
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int hh = 0; hh < 2; hh++) {
-                    sc[n][hh] *= mul[n][hh];
-                    sc[n][2 + hh] *= mul[n][hh];
-                }
-            if (tok0 + kKv4Tokens > low) {   // some column does not see all of the page
-#pragma unroll
-                for (int n = 0; n < NT; n++)
+                    mma_f16_16816(c, higha, qh[n][b][2], qh[n][b][3]);
 #pragma unroll
                     for (int hh = 0; hh < 2; hh++) {
-                        if (tok0 + g >= lim[n][hh]) sc[n][hh] = -CUDART_INF_F;
-                        if (tok0 + g + 8 >= lim[n][hh]) sc[n][2 + hh] = -CUDART_INF_F;
+                        sc[p][n][hh] = fmaf(d0, fmaf(-z0, qs[n][hh][b], c[hh]), sc[p][n][hh]);
+                        sc[p][n][2 + hh] = fmaf(d1, fmaf(-z1, qs[n][hh][b], c[2 + hh]), sc[p][n][2 + hh]);
                     }
+                }
             }
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int hh = 0; hh < 2; hh++)
-                    over |= fmaxf(sc[n][hh], sc[n][2 + hh]) > base[n][hh] + 8.0f;
-            if (__any_sync(0xffffffffu, over)) {
+                for (int k = 0; k < 4; k++) {
+                    if (PACK) sc[p][n][k] += __shfl_xor_sync(0xffffffffu, sc[p][n][k], 2);
+                    sc[p][n][k] *= mul[n][k & 1];
+                }
+            if (tok0[p] + kKv4Tokens > low) {   // some column does not see all of the page
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int hh = 0; hh < 2; hh++) {
-                        float mx = fmaxf(sc[n][hh], sc[n][2 + hh]);
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        if (mx > base[n][hh]) {
-                            const float f = ex2(base[n][hh] - mx);   // 0 from -inf
-                            base[n][hh] = mx;
-                            l[n][hh] *= f;
-#pragma unroll
-                            for (int m = 0; m < MT; m++) {
-                                o[n][m][hh] *= f;
-                                o[n][m][2 + hh] *= f;
-                            }
-                        }
-                    }
+                    for (int k = 0; k < 4; k++)
+                        if (tok0[p] + g + 4 * (k & 2) >= lim[n][k & 1]) sc[p][n][k] = -CUDART_INF_F;
             }
-            // weights, as P^T operands: tokens 2t, 2t + 1 and + 8, column g
-            uint32_t ph[NT][2], pl[NT][2];
+        }
+        float mx[NT][2];
+        bool over = false;
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float p[4];
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+                mx[n][hh] = fmaxf(sc[0][n][hh], sc[0][n][2 + hh]);
+#pragma unroll
+                for (int p = 1; p < PP; p++)
+                    mx[n][hh] = fmaxf(mx[n][hh], fmaxf(sc[p][n][hh], sc[p][n][2 + hh]));
+                over |= mx[n][hh] > base[n][hh] + 8.0f;
+            }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int hh = 0; hh < 2; hh++) {
-                    const float b7 = base[n][hh] == -CUDART_INF_F ? 0.0f : base[n][hh] - 7.0f;
-                    p[hh] = ex2(sc[n][hh] - b7);
-                    p[2 + hh] = ex2(sc[n][2 + hh] - b7);
-                    l[n][hh] += p[hh] + p[2 + hh];
-                }
-                uint32_t h0, l0, h1, l1;
-                split2(p[0], p[1], h0, l0);
-                split2(p[2], p[3], h1, l1);
-                ph[n][0] = movmatrix_t(h0);
-                ph[n][1] = movmatrix_t(h1);
-                pl[n][0] = movmatrix_t(l0);
-                pl[n][1] = movmatrix_t(l1);
-            }
-            // steps and zero points of tokens (2t, 2t + 1) and (2t + 8, 2t + 9)
-            uint32_t d2[2][NB], z2[2][NB], z2h[2][NB];
+                    float m = mx[n][hh];
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    m = fmaxf(m, base[n][hh]);
+                    const float f = m == -CUDART_INF_F ? 1.0f : ex2(base[n][hh] - m);   // 0 from -inf
+                    base[n][hh] = m;
+                    l[n][hh] *= f;
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                Scales<NB> sa, sb;
-                sa.load(pg + F::VS, 2 * t + 8 * u);
-                sb.load(pg + F::VS, 2 * t + 1 + 8 * u);
-                if (tok0 + kKv4Tokens > ctx) {   // slots behind the last token: any bits
-#pragma unroll
-                    for (int w = 0; w < Scales<NB>::W; w++) {
-                        if (tok0 + 2 * t + 8 * u >= ctx) sa.w[w] = 0;
-                        if (tok0 + 2 * t + 1 + 8 * u >= ctx) sb.w[w] = 0;
+                    for (int k = 0; k < MT; k++) {
+                        o[n][k][hh] *= f;
+                        o[n][k][2 + hh] *= f;
                     }
                 }
+        }
+        __syncwarp();   // V factors are written
+        // weights, as P^T operands: tokens 2t, 2t + 1 and + 8, column g
+        uint32_t ph[PP][NT][2], pl[PP][PACK ? 1 : NT][2];
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const uint32_t w = __byte_perm(sa.word(b), sb.word(b), b & 1 ? 0x7632 : 0x5410);
-                    d2[u][b] = w & 0x7ff07ff0u;
-                    z2[u][b] = (w & 0x000f000fu) | 0x64006400u;           // 1024 + z
-                    z2h[u][b] = ((w << 4) & 0x00f000f0u) | 0xd400d400u;   // -(64 + z)
+        for (int n = 0; n < NT; n++) {
+            float b7[2];
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) b7[hh] = base[n][hh] == -CUDART_INF_F ? 0.0f : base[n][hh] - 7.0f;
+#pragma unroll
+            for (int p = 0; p < PP; p++) {
+                float w[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[k] = ex2(sc[p][n][k] - b7[k & 1]);
+                l[n][0] += w[0] + w[2];
+                l[n][1] += w[1] + w[3];
+                if constexpr (PACK) {   // the high parts (t < 2), or what they leave
+                    const float2 a0 = f16_pair(pack_f16(w[0], w[1])), a1 = f16_pair(pack_f16(w[2], w[3]));
+                    ph[p][n][0] = movmatrix_t(pack_f16(fmaf(rest, a0.x, w[0]), fmaf(rest, a0.y, w[1])));
+                    ph[p][n][1] = movmatrix_t(pack_f16(fmaf(rest, a1.x, w[2]), fmaf(rest, a1.y, w[3])));
+                } else {
+                    uint32_t h0, l0, h1, l1;
+                    split2(w[0], w[1], h0, l0);
+                    split2(w[2], w[3], h1, l1);
+                    ph[p][n][0] = movmatrix_t(h0);
+                    ph[p][n][1] = movmatrix_t(h1);
+                    pl[p][n][0] = movmatrix_t(l0);
+                    pl[p][n][1] = movmatrix_t(l1);
                 }
             }
-            // O^T += V^T P^T
-            constexpr int TPG = F::TPG;
+        }
+        // O^T += V^T P^T.  A product truncates what it adds to about 24 bits of the
+        // largest term, so a step's products are summed from zero and added in
+        // fp32: the error does not grow with the number of pages.
+        constexpr int TPG = F::TPG;
+        uint32_t f2[PP][4], dh[PP][2];   // D and Z of tokens (2t, 2t + 1), (2t + 8, 2t + 9), D / 16
 #pragma unroll
-            for (int m0 = 0; m0 < MT; m0 += TPG) {
-                uint32_t w[TPG];
-                lds_words<TPG>(w, pg + F::V + (m0 / TPG) * (128 * TPG) + lane * (4 * TPG));
+        for (int m0 = 0; m0 < MT; m0 += TPG) {
+            uint32_t x[PP][TPG];
 #pragma unroll
-                for (int k = 0; k < TPG; k++) {
-                    const int m = m0 + k, b = m / 2;
-                    const uint32_t x = w[k], y = w[k] >> 8;
+            for (int p = 0; p < PP; p++)
+                lds_words<TPG>(x[p], buf + p * F::BYTES + F::V + (m0 / TPG) * (128 * TPG) + lane * (4 * TPG));
+#pragma unroll
+            for (int k = 0; k < TPG; k++) {
+                const int m = m0 + k, b = m / 2;
+                float c[NT][4];
+#pragma unroll
+                for (int p = 0; p < PP; p++) {
+                    if (m % 2 == 0) {
+                        lds_words<4>(f2[p], vsc + p * C::VSC_PAGE + (t * NB + b) * 16);
+                        dh[p][0] = hmul2u(f2[p][0], 0x2c002c00u);
+                        dh[p][1] = hmul2u(f2[p][2], 0x2c002c00u);
+                    }
                     uint32_t v[4];
-                    v[0] = hmul2u(hsub2u((x & 0x000f000fu) | 0x64006400u, z2[0][b]), d2[0][b]);
-                    v[1] = hmul2u(hfma2u((x & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z2h[0][b]), d2[0][b]);
-                    v[2] = hmul2u(hsub2u((y & 0x000f000fu) | 0x64006400u, z2[1][b]), d2[1][b]);
-                    v[3] = hmul2u(hfma2u((y & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z2h[1][b]), d2[1][b]);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint32_t y = u ? x[p][k] >> 8 : x[p][k], D = f2[p][2 * u], Z = f2[p][2 * u + 1];
+                        v[2 * u] = hfma2u(y & 0x000f000fu, D, Z);
+                        v[2 * u + 1] = hfma2u(y & 0x00f000f0u, dh[p][u], Z);
+                    }
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        mma_f16_16816(o[n][m], v, ph[n][0], ph[n][1]);
-                        mma_f16_16816(o[n][m], v, pl[n][0], pl[n][1]);
+                        if constexpr (PACK) {
+                            if (p == 0) mma_f16_16816_first(c[n], v, ph[p][n][0], ph[p][n][1]);
+                            else mma_f16_16816(c[n], v, ph[p][n][0], ph[p][n][1]);
+                        } else {
+                            if (p == 0) mma_f16_16816_first(c[n], v, pl[p][n][0], pl[p][n][1]);
+                            else mma_f16_16816(c[n], v, pl[p][n][0], pl[p][n][1]);
+                            mma_f16_16816(c[n], v, ph[p][n][0], ph[p][n][1]);
+                        }
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[n][m][j] += c[n][j];
             }
         }
         __syncwarp();   // buffer s is read
-        if (it + NBUF < npw) issue(it + NBUF);
+        if (it + NBUF < part_steps) issue(part, it + NBUF);
     }
 
-    // the warp's state to shared memory
+    // the warp's state to shared memory, O without the V factors' 2^(e - 24)
+    const float unscale = __uint_as_float((uint32_t)(127 + 24 - dexp) << 23);
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[n][m][k] *= unscale;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -443,110 +813,73 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) kv4_attn_narrow_kernel(cons
             l[n][hh] += __shfl_xor_sync(0xffffffffu, l[n][hh], 8);
             l[n][hh] += __shfl_xor_sync(0xffffffffu, l[n][hh], 16);
         }
-    __syncthreads();   // every ring is read
-    float* acc_s = reinterpret_cast<float*>(nar_sm);                       // [W][COLS][PITCH]
-    float* ml_s = acc_s + (size_t)W * C::COLS * C::PITCH;                  // [W][COLS][2]
+    if (PACK)
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+        for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int hh = 0; hh < 2; hh++) {
-            const int col = 8 * n + 2 * t + hh;
-            float* row = acc_s + ((size_t)warp * C::COLS + col) * C::PITCH;
+            for (int k = 0; k < 4; k++) o[0][m][k] += __shfl_xor_sync(0xffffffffu, o[0][m][k], 2);
+    // the next part's first copies land while this one is written
+    used += part_steps;
+    const bool more = next.b1 > next.b0;
+    if (more) {
+        for (int n = 0; n < min(steps_of(next), NBUF); n++) issue(next, n);
+        fetch_q(next, qb ^ 1);
+    }
+    __syncthreads();   // the states of the last part are read
+    if (threadIdx.x == 0 && more)
+        narrow_next_part<COLS>(a, kept, run_s, parts[which == 0 ? 2 : which - 1]);
+    if (!PACK || t < 2) {
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                row[16 * m + g] = o[n][m][hh];
-                row[16 * m + g + 8] = o[n][m][2 + hh];
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+                const int col = 8 * n + tq + hh;
+                float* row = acc_s + ((size_t)warp * COLS + col) * C::PITCH;
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    row[16 * m + g] = o[n][m][hh];
+                    row[16 * m + g + 8] = o[n][m][2 + hh];
+                }
+                if (g == 0) {
+                    ml_s[(warp * COLS + col) * 2] = base[n][hh];
+                    ml_s[(warp * COLS + col) * 2 + 1] = l[n][hh];
+                }
             }
-            if (g == 0) {
-                ml_s[(warp * C::COLS + col) * 2] = base[n][hh];
-                ml_s[(warp * C::COLS + col) * 2 + 1] = l[n][hh];
-            }
-        }
-    __syncthreads();
-    const int live = min(C::COLS, cols - col0);
-    float* pacc = a.part + ((int64_t)tile * a.nsplit + sp) * C::COLS * HD;
-    float* pml = a.part + (int64_t)gridDim.x * gridDim.y * a.nsplit * C::COLS * HD +
-                 ((int64_t)tile * a.nsplit + sp) * C::COLS * 2;
+    }
+    cp_async_wait_all();
+    __syncthreads();   // states, and the next part's Q
+    const int c0 = part.c0, c1 = part.c1, live = min(COLS, part.cols - part.col0);
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (c0 == (int)blockIdx.x);
     for (int idx = threadIdx.x; idx < live * (HD / 4); idx += W * 32) {
         const int col = idx / (HD / 4), d = idx % (HD / 4) * 4;
         float mx = -CUDART_INF_F;
 #pragma unroll
-        for (int w = 0; w < W; w++) mx = fmaxf(mx, ml_s[(w * C::COLS + col) * 2]);
+        for (int w = 0; w < W; w++) mx = fmaxf(mx, ml_s[(w * COLS + col) * 2]);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; w++) {
-            const float mw = ml_s[(w * C::COLS + col) * 2];
+            const float mw = ml_s[(w * COLS + col) * 2];
             const float f = mw == -CUDART_INF_F ? 0.0f : ex2(mw - mx);
-            const float4 x = *reinterpret_cast<const float4*>(acc_s + ((size_t)w * C::COLS + col) * C::PITCH + d);
+            const float4 x = *reinterpret_cast<const float4*>(acc_s + ((size_t)w * COLS + col) * C::PITCH + d);
             v.x = fmaf(x.x, f, v.x);
             v.y = fmaf(x.y, f, v.y);
             v.z = fmaf(x.z, f, v.z);
             v.w = fmaf(x.w, f, v.w);
-            sum = fmaf(ml_s[(w * C::COLS + col) * 2 + 1], f, sum);
+            sum = fmaf(ml_s[(w * COLS + col) * 2 + 1], f, sum);
         }
-        if (ns > 1) {
-            *reinterpret_cast<float4*>(pacc + col * HD + d) = v;
-            if (d == 0) {
-                pml[col * 2] = mx;
-                pml[col * 2 + 1] = sum;
-            }
-            continue;
+        if (c1 > c0) {
+            *reinterpret_cast<float4*>(a.part + (slot * COLS + col) * HD + d) = v;
+            if (d == 0)
+                *reinterpret_cast<float2*>(a.part + (int64_t)gridDim.x * 2 * COLS * HD + (slot * COLS + col) * 2) =
+                    make_float2(mx, sum);
+        } else {
+            narrow_write(a, part, HD, col, d, v, sum);
         }
-        const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;   // nothing seen: zeros
-        const int c = col0 + col, j = c / a.G;
-        *reinterpret_cast<float4*>(a.out + (int64_t)(r0 + j) * a.n_heads * HD +
-                                   (int64_t)(kvh * a.G + c - j * a.G) * HD + d) =
-            make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
     }
-    if (ns == 1) return;
-
-    // the last split's CTA joins them, in split order
-    __threadfence();
-    __syncthreads();
-    __shared__ int last;
-    if (threadIdx.x == 0) {
-        last = atomicAdd(a.counters + tile, 1) == ns - 1;
-        if (last) a.counters[tile] = 0;
-    }
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    pacc = a.part + (int64_t)tile * a.nsplit * C::COLS * HD;
-    pml = a.part + (int64_t)gridDim.x * gridDim.y * a.nsplit * C::COLS * HD + (int64_t)tile * a.nsplit * C::COLS * 2;
-    float* fac = acc_s;                      // [ns][COLS] factors, then [COLS] 1 / sum
-    for (int col = warp; col < live; col += W) {
-        float mx = -CUDART_INF_F, sum = 0.0f;
-        for (int k = lane; k < ns; k += 32) mx = fmaxf(mx, __ldcg(pml + ((int64_t)k * C::COLS + col) * 2));
-        mx = warp_max(mx);
-        for (int k = lane; k < ns; k += 32) {
-            const float mk = __ldcg(pml + ((int64_t)k * C::COLS + col) * 2);
-            const float f = mk == -CUDART_INF_F ? 0.0f : ex2(mk - mx);
-            fac[k * C::COLS + col] = f;
-            sum = fmaf(__ldcg(pml + ((int64_t)k * C::COLS + col) * 2 + 1), f, sum);
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) fac[ns * C::COLS + col] = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
-    }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < live * (HD / 4); idx += W * 32) {
-        const int col = idx / (HD / 4), d = idx % (HD / 4) * 4;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int k = 0; k < ns; k++) {
-            const float f = fac[k * C::COLS + col];
-            const float4 x = ld_cg4(pacc + ((int64_t)k * C::COLS + col) * HD + d);
-            v.x = fmaf(x.x, f, v.x);
-            v.y = fmaf(x.y, f, v.y);
-            v.z = fmaf(x.z, f, v.z);
-            v.w = fmaf(x.w, f, v.w);
-        }
-        const float inv = fac[ns * C::COLS + col];
-        const int c = col0 + col, j = c / a.G;
-        *reinterpret_cast<float4*>(a.out + (int64_t)(r0 + j) * a.n_heads * HD +
-                                   (int64_t)(kvh * a.G + c - j * a.G) * HD + d) =
-            make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    }
+    if (c1 > c0 && c0 == (int)blockIdx.x && threadIdx.x == 0) a.split[blockIdx.x] = part;
+    if (!more) break;
+  }
 }
 
 }  // namespace axq8

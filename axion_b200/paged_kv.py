@@ -149,9 +149,9 @@ class PagedKVCache4:
     manages; sequences and positions are then named by the caller
     (``append_rows``, ``decode_attention``, ``chunk_attention``).
 
-    Calls go to the current stream of the cache's device; calls of one cache
-    on several streams have their own workspaces, and so has every captured
-    graph.
+    Calls go to the current stream of the cache's device.  Workspaces come from
+    torch's allocator, a call's own: calls of one cache on several streams and
+    captured graphs may run at once.
     """
 
     page_size = 16
@@ -192,7 +192,6 @@ class PagedKVCache4:
                                     self.max_blocks, pages.shape[0], n_kv_heads, head_dim,
                                     self.page_size)
         self._ref = C.byref(self.c)
-        self._ws: dict[int, torch.Tensor] = {}
         self._need: dict[tuple, int] = {}
         self._lib = _lib.load()
 
@@ -233,14 +232,7 @@ class PagedKVCache4:
         if need < 0:
             raise RuntimeError(_lib.load().axq8_last_error().decode(errors="replace")
                                or "PagedKVCache4: unsupported attention shape")
-        if torch.cuda.is_current_stream_capturing():
-            # a graph keeps its own: it may be replayed beside any other call
-            return torch.zeros(need, dtype=torch.uint8, device=self.pages.device)
-        stream = torch.cuda.current_stream(self.pages.device).cuda_stream
-        ws = self._ws.get(stream)
-        if ws is None or ws.numel() < need:
-            ws = self._ws[stream] = torch.zeros(need, dtype=torch.uint8, device=self.pages.device)
-        return ws
+        return torch.empty(need, dtype=torch.uint8, device=self.pages.device)
 
     def _stream(self) -> int:
         return torch.cuda.current_stream(self.pages.device).cuda_stream

@@ -141,9 +141,8 @@ int64_t axkv4_decode_attn_workspace(const axkv4_cache_t* c, int32_t n_rows, int3
  * row with q_pos < 0 attends to nothing and gives zeros (padding of a batch).
  * Pages whose id is outside the pool count as masked and are reported in the
  * status word, as are sequences and positions outside the table.  n_heads a
- * multiple of n_kv_heads, at most 16 times as many.  The workspace must be
- * zero before its first use and serves calls of any size after; calls sharing
- * a workspace must not overlap on the GPU. */
+ * multiple of n_kv_heads, at most 16 times as many.  The workspace's
+ * contents need not be set; calls sharing it must not overlap on the GPU. */
 int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_t n_rows,
                       int32_t n_heads, const int32_t* q_seq, const int32_t* q_pos, float* out,
                       void* workspace, int64_t workspace_bytes, void* stream);
