@@ -13,6 +13,7 @@
 #include "common.cuh"
 #include "kv4.cuh"
 #include "kv4_narrow.cuh"
+#include "kv4_wide.cuh"
 #include "runtime.h"
 
 using namespace axq8;
@@ -242,6 +243,37 @@ cudaError_t launch_narrow(const NarrowPlan& p, const axkv4_cache_t* c, const flo
                          : launch_narrow_cols<HD, 16>(a, p.ctas, s);
 }
 
+template <int HD>
+cudaError_t launch_wide(const axkv4_cache_t* c, const float* q, int64_t ldq, int n_rows, int chunks,
+                        int max_rows, int n_heads, const int* q_seq, const int* q_start,
+                        const int* q_pos, float* out, int* status, cudaStream_t s) {
+    WideArgs a = {};
+    a.c = pages_of(c);
+    a.q = q;
+    a.ldq = ldq;
+    a.n_rows = n_rows;
+    a.max_rows = max_rows;
+    a.n_heads = n_heads;
+    a.G = n_heads / c->n_kv_heads;
+    a.q_seq = q_seq;
+    a.q_start = q_start;
+    a.q_pos = q_pos;
+    a.scale = 1.4426950408889634f / std::sqrt((float)HD);
+    a.out = out;
+    a.status = status;
+    constexpr size_t smem = WideCfg<HD>::SMEM;
+    const cudaError_t e = cudaFuncSetAttribute(kv4_attn_wide_kernel<HD>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    const int64_t rows = (int64_t)std::min(max_rows, n_rows) * a.G;
+    return launch_k(kv4_attn_wide_kernel<HD>, dim3((unsigned)((rows + 255) / 256), c->n_kv_heads, chunks),
+                    dim3(kWideThreads), smem, s, false, a);
+}
+
+// Columns (rows x heads of a KV head) of a chunk from which the tensor-core
+// tiles of 128 rows take it.
+constexpr int kWideCols = 33;
+
 }  // namespace
 
 extern "C" {
@@ -315,6 +347,7 @@ int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32
 int64_t axkv4_chunk_attn_workspace(const axkv4_cache_t* c, int32_t n_chunks, int32_t max_rows,
                                    int32_t n_heads) {
     if (check_attn(c, "axkv4_chunk_attn_workspace", n_heads) || n_chunks <= 0 || max_rows <= 0) return -1;
+    if ((int64_t)max_rows * (n_heads / c->n_kv_heads) >= kWideCols) return 16;
     DeviceState* ds = device_state();
     if (!ds) return -1;
     return narrow_plan(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads).workspace;
@@ -341,6 +374,14 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
     if (workspace_bytes <= 0) return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: no workspace");
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
+    if ((int64_t)max_rows * (n_heads / c->n_kv_heads) >= kWideCols) {
+        if (c->n_kv_heads > 65535) return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d KV heads", c->n_kv_heads);
+        AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_wide, c, q, ldq, n_rows, n_chunks, max_rows, n_heads,
+                                      q_seq, q_start, q_pos, out, ds->status,
+                                      static_cast<cudaStream_t>(stream)),
+                      "axkv4_chunk_attn launch");
+        return AXQ8_OK;
+    }
     const NarrowPlan p = narrow_plan(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads);
     if (p.units > 0x7fffffff)
         return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d chunks of %d rows, %d pages", n_chunks,

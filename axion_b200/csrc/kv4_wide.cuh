@@ -1,0 +1,504 @@
+// Causal attention of long chunks over the 4-bit cache on the 5th-generation
+// tensor cores (tcgen05.mma kind::f16, accumulators in TMEM).
+//
+// The (row, head) pairs that read one KV head of one chunk are the rows of
+// 128-row tiles; a CTA takes two tiles (256 rows: 64 positions of 4 heads) and
+// walks the tokens 0 .. its last position in steps of 128 (8 pages):
+//   S [128 x 128] = Q K^T     A = Q from shared memory, B = K
+//   O [128 x HD] += P V       A = P from TMEM, B = V^T
+// A cache value d (q - z) is an fp16 number, so K and V^T tiles are formed in
+// shared memory without rounding (128-byte-swizzled K-major rows), once for
+// both tiles.  Q (scaled per row by a power of two to below 2^14) and P (2^7
+// times the softmax weight) are an fp16 high part plus an fp16 residual,
+// multiplied one after the other: results keep fp32 accuracy at twice the
+// products.  Dims within 8 stand in the order 0 4 1 5 2 6 3 7 in both Q and K:
+// the order in which a code word's nibbles come out in pairs.
+//
+// Roles: warps 0-3 and 4-7 the softmax of tile 0 and 1 (a thread is a row),
+// warps 8-11 form the K and V^T tiles from page words that they read a step
+// ahead, warp 12 issues the products in the order
+//   PV(tile 0, step j)  QK(tile 0, j + 1)  PV(tile 1, j)  QK(tile 1, j + 1)
+// so that each tile's softmax runs under the other tile's products.  P takes
+// the place of S in TMEM, 32 tokens at a time.  The softmax reference moves (and
+// O is rescaled) only when a score exceeds it by more than 8 (base 2).
+//
+// Bound: 4 x 128 x 128 x HD multiply-adds a step and tile.  Every wait is
+// bounded; a role that gives up raises a flag, and all stop.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "kv4.cuh"
+#include "kv4_narrow.cuh"
+#include "tcgen05.cuh"
+
+namespace axq8 {
+
+constexpr int kWideTok = 128;                      // tokens of a step
+constexpr int kWidePages = kWideTok / kKv4Tokens;
+constexpr int kWideThreads = 13 * 32;
+
+struct WideArgs {
+    Kv4Pages c;
+    const float* q;
+    int64_t ldq;
+    int n_rows, max_rows, n_heads, G;
+    const int* q_seq;
+    const int* q_start;
+    const int* q_pos;
+    float scale;          // softmax scale times log2(e)
+    float* out;
+    int* status;
+};
+
+template <int HD>
+struct WideCfg {
+    static constexpr int ATOMS = HD > 64 ? 2 : 1;           // 64 dims of a Q or K row
+    static constexpr int ATOM = kWideTok * 128;             // bytes: 128 rows of 128
+    static constexpr int Q = 2 * 2 * ATOMS * ATOM;          // [tile][high, residual][atom]
+    static constexpr int K = ATOMS * ATOM;
+    static constexpr int VATOM = HD * 128;                  // 64 tokens of a V^T row
+    static constexpr int V = 2 * VATOM;
+    static constexpr int OFF_K = Q, OFF_V = Q + K;
+    static constexpr int OFF_VS = OFF_V + V;                // V scales [2][page][block][16]
+    static constexpr int VS = kWidePages * (HD / 32) * 32;
+    static constexpr int OFF_BAR = OFF_VS + 2 * VS;
+    static constexpr int SMEM = 1024 + OFF_BAR + 256;
+    static constexpr int TILE_COLS = 128 + (HD < 32 ? 32 : HD);   // S (P), then O
+    static constexpr int TMEM_COLS = 512;
+};
+
+// Instruction descriptor, kind::f16: D fp32 (bits 4-5 = 1), A and B fp16, both
+// K-major, N >> 3 at bit 17, M >> 4 at bit 24.
+__host__ __device__ constexpr uint32_t wide_idesc(int M, int N) {
+    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+        "%29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// 8 codes of a word as 4 fp16 pairs (q0 q4) (q1 q5) (q2 q6) (q3 q7), minus the
+// zero points z (1024 + z pair), zh (-(64 + z) pair), times the steps d.
+__device__ __forceinline__ void kv4_word(uint32_t w, uint32_t d, uint32_t z, uint32_t zh, uint32_t* v) {
+    const uint32_t y = w >> 8;
+    v[0] = hmul2u(hsub2u((w & 0x000f000fu) | 0x64006400u, z), d);
+    v[1] = hmul2u(hfma2u((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, zh), d);
+    v[2] = hmul2u(hsub2u((y & 0x000f000fu) | 0x64006400u, z), d);
+    v[3] = hmul2u(hfma2u((y & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, zh), d);
+}
+
+// Wait for a phase; false (and all roles stop) when it does not come, or when
+// another role has given up.
+__device__ __forceinline__ bool wide_wait(uint64_t* bar, uint32_t parity, volatile int* stop, int* status) {
+    for (int i = 0; i < 200000; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(10000)
+            : "memory");
+        if (ok) return true;
+        if (*stop) return false;
+    }
+    *stop = 1;
+    record_status(status, AXQ8_ERR_WAIT_TIMEOUT);
+    return false;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __grid_constant__ WideArgs a) {
+    using F = Kv4<HD>;
+    using C = WideCfg<HD>;
+    constexpr int NB = F::NB;
+    extern __shared__ uint8_t wide_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wide_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+    uint64_t *kfull = bars, *vfull = bars + 1, *kfree = bars + 2, *vfree = bars + 3, *qfull = bars + 4,
+             *sfull = bars + 5, *pfull = bars + 7, *odone = bars + 9;   // sfull, pfull: [tile]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 10);
+    volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(tmem_slot + 2);   // [2] pages of a step
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // the chunk's rows and positions; the last tiles, with the most tokens, first
+    const int i = blockIdx.z, kvh = blockIdx.y;
+    const int r0 = a.q_start[i], T = a.q_start[i + 1] - r0;
+    if (T <= 0) return;
+    if (r0 < 0 || r0 > a.n_rows - T || T > a.max_rows) {
+        if (threadIdx.x == 0) record_status(a.status, AXQ8_ERR_INVALID);
+        return;
+    }
+    const int rows = T * a.G, m0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * 256;
+    if (m0 >= rows) return;
+    const int room = a.c.max_blocks * kKv4Tokens;
+    const int seq_in = a.q_seq ? a.q_seq[i] : i;
+    const bool seq_ok = seq_in >= 0 && seq_in < a.c.n_seqs;
+    const int seq = seq_ok ? seq_in : 0, pos0 = min(a.q_pos[i], room);
+    if ((!seq_ok || pos0 + T > room) && threadIdx.x == 0 && m0 == 0) record_status(a.status, AXQ8_ERR_INVALID);
+    const int tiles = rows - m0 > 128 ? 2 : 1;
+    const int jlast = min(rows - 1, m0 + 255) / a.G;
+    const int ctx = seq_ok ? max(0, min(pos0 + jlast + 1, room)) : 0;
+    const int steps = max(1, (ctx + kWideTok - 1) / kWideTok);
+
+    if (threadIdx.x == 0) {
+        mbar_init(kfull, 128);
+        mbar_init(vfull, 128);
+        mbar_init(kfree, 1);
+        mbar_init(vfree, 1);
+        mbar_init(qfull, 128 * tiles);
+        for (int x = 0; x < 2; x++) {
+            mbar_init(sfull + x, 1);
+            mbar_init(pfull + x, 128);
+        }
+        mbar_init(odone, 1);
+        *stop = 0;
+        fence_mbar_init();
+    }
+    if (warp == 12) tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp < 8) {
+        // ---- softmax: thread = row of tile x --------------------------------------
+        const int x = warp >> 2;
+        if (x < tiles) {
+            const int r = (warp & 3) * 32 + lane, m = m0 + 128 * x + r;
+            const bool live = m < rows;
+            const int j = min(m, rows - 1) / a.G, head = kvh * a.G + min(m, rows - 1) - j * a.G;
+            const float* qp = a.q + (int64_t)(r0 + j) * a.ldq + (int64_t)head * HD;
+            float mx = 0.0f;
+            for (int d = 0; d < HD; d += 4) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(qp + d));
+                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            }
+            // 2^k with max |q| 2^k in [2^13, 2^14)
+            const int ex = max((int)(__float_as_uint(mx) >> 23), 40) - 127;
+            const float up = live ? __uint_as_float((uint32_t)(127 + 13 - ex) << 23) : 0.0f;
+            const float mul = __uint_as_float((uint32_t)(127 - 13 + ex) << 23) * a.scale;
+            uint8_t* qs = sm + x * 2 * C::ATOMS * C::ATOM;
+#pragma unroll 2
+            for (int ch = 0; ch < HD / 8; ch++) {
+                const float4 u = __ldg(reinterpret_cast<const float4*>(qp + 8 * ch));
+                const float4 v = __ldg(reinterpret_cast<const float4*>(qp + 8 * ch + 4));
+                uint4 hi, lo;
+                split2(u.x * up, v.x * up, hi.x, lo.x);
+                split2(u.y * up, v.y * up, hi.y, lo.y);
+                split2(u.z * up, v.z * up, hi.z, lo.z);
+                split2(u.w * up, v.w * up, hi.w, lo.w);
+                uint8_t* at = qs + (ch >> 3) * C::ATOM + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                *reinterpret_cast<uint4*>(at) = hi;
+                *reinterpret_cast<uint4*>(at + C::ATOMS * C::ATOM) = lo;
+            }
+            fence_async_smem();
+            mbar_arrive(qfull);
+
+            const int pos = live && seq_ok ? min(pos0 + j, room - 1) : -1;   // the last token seen
+            const int sees = __reduce_min_sync(0xffffffffu, live ? pos : 0x7fffffff);
+            const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * C::TILE_COLS, to = ts + 128;
+            float base = -CUDART_INF_F, l = 0.0f;
+            uint32_t s[32];
+            bool ok = true;
+            for (int st = 0; st < steps; st++) {
+                if (!__all_sync(0xffffffffu, wide_wait(sfull + x, st & 1, stop, a.status))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const int tok0 = st * kWideTok;
+                const uint32_t pages = present[st & 1];
+                const bool whole = tok0 + kWideTok - 1 <= sees && pages == (1u << kWidePages) - 1;
+                auto load = [&](int c) {
+                    tmem_ld32(ts + 32 * c, s);
+                    tmem_wait_ld32(s);
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            const int tok = 32 * c + e;
+                            if (tok0 + tok > pos || !((pages >> (tok / kKv4Tokens)) & 1)) s[e] = 0xff800000u;
+                        }
+                    }
+                };
+                float top = -CUDART_INF_F;
+#pragma unroll 1
+                for (int c = 0; c < kWideTok / 32; c++) {
+                    load(c);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(s[e]));
+                }
+                top *= mul;
+                const bool over = top > base + 8.0f;
+                if (__any_sync(0xffffffffu, over)) {
+                    const float f = over ? ex2(base - top) : 1.0f;   // 0 from -inf
+                    if (over) base = top;
+                    l *= f;
+                    if (st) {
+#pragma unroll 1
+                        for (int c = 0; c < HD / 32; c++) {
+                            tmem_ld32(to + 32 * c, s);
+                            tmem_wait_ld32(s);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) s[e] = __float_as_uint(__uint_as_float(s[e]) * f);
+                            tmem_st32(to + 32 * c, s);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                const float b7 = base == -CUDART_INF_F ? 0.0f : base - 7.0f;
+#pragma unroll 1
+                for (int c = 0; c < kWideTok / 32; c++) {
+                    load(c);
+                    uint32_t pw[32];   // columns: 16 high pairs, then 16 residual pairs
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float w0 = ex2(fmaf(__uint_as_float(s[2 * e]), mul, -b7));
+                        const float w1 = ex2(fmaf(__uint_as_float(s[2 * e + 1]), mul, -b7));
+                        l += w0 + w1;
+                        split2(w0, w1, pw[e], pw[16 + e]);
+                    }
+                    tmem_st32(ts + 32 * c, pw);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(pfull + x);
+            }
+            // O / l
+            if (ok && __all_sync(0xffffffffu, wide_wait(odone, 0, stop, a.status))) {
+                tc_fence_after();
+                const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;   // nothing seen: zeros
+                float* op = a.out + (int64_t)(r0 + j) * a.n_heads * HD + (int64_t)head * HD;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; c++) {
+                    tmem_ld32(to + 32 * c, s);
+                    tmem_wait_ld32(s);
+                    if (live) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4*>(op + 32 * c + e) =
+                                make_float4(__uint_as_float(s[e]) * inv, __uint_as_float(s[e + 1]) * inv,
+                                            __uint_as_float(s[e + 2]) * inv, __uint_as_float(s[e + 3]) * inv);
+                    }
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ---- K and V^T tiles ------------------------------------------------------
+        const int w = warp - 8, th = threadIdx.x - 256;
+        constexpr int VT = HD / 2, VI = HD / 32;           // threads of a page's V, pages of a thread
+        const int vp = th / VT, vm = (th % VT) / 8, vg = th % 8;
+        const int* row = a.c.table + (int64_t)seq * a.c.max_blocks;
+        uint32_t kw[4][NB], vw[VI][4], present_now = 0;
+        Scales<NB> ksc[4], vsc;
+        int ids = -1;
+        auto page_ids = [&](int st) {      // lane p: page p of step st
+            const int blk = st * kWidePages + (lane & 7);
+            const bool in = blk * kKv4Tokens < ctx;
+            ids = in ? __ldg(row + blk) : -1;
+            const bool bad = (unsigned)ids >= (unsigned)a.c.n_pages;
+            if (bad) {
+                if (in && lane < 8) record_status(a.status, AXQ8_ERR_INVALID);
+                ids = -1;
+            }
+            present_now = __ballot_sync(0xffffffffu, lane < 8 && ids >= 0);
+        };
+        auto page_at = [&](int p) {
+            const int id = __shfl_sync(0xffffffffu, ids, p);
+            return id < 0 ? nullptr : a.c.pages + ((int64_t)id * a.c.n_kv + kvh) * F::BYTES;
+        };
+        auto read_k = [&](int st) {        // tokens 32 w + 8 k + lane / 4, chunk lane % 4
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int tok = 32 * w + 8 * k + (lane >> 2), slot = tok % kKv4Tokens;
+                const uint8_t* pg = page_at(tok / kKv4Tokens);
+                const bool in = pg && st * kWideTok + tok < ctx;
+#pragma unroll
+                for (int b = 0; b < NB; b++) kw[k][b] = 0;
+#pragma unroll
+                for (int b = 0; b < Scales<NB>::W; b++) ksc[k].w[b] = 0;
+                if (in) {
+                    lds_words<NB>(kw[k], pg + slot * (HD / 2) + (lane & 3) * (HD / 8));
+                    ksc[k].load(pg + F::KS, slot);
+                }
+            }
+        };
+        auto read_v = [&](int st) {
+#pragma unroll
+            for (int k = 0; k < VI; k++) {
+                const uint8_t* pg = page_at(vp + k * (kWidePages / VI));
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    vw[k][t] = pg ? __ldg(reinterpret_cast<const uint32_t*>(
+                                        pg + F::V + (vm / F::TPG) * (128 * F::TPG) + (vg * 4 + t) * (4 * F::TPG) +
+                                        (vm % F::TPG) * 4))
+                                  : 0u;
+            }
+            const uint8_t* pg = page_at(th / kKv4Tokens % kWidePages);
+            // the scales of token th; slots behind the last token hold any bits
+#pragma unroll
+            for (int b = 0; b < Scales<NB>::W; b++) vsc.w[b] = 0;
+            if (pg && st * kWideTok + th < ctx) vsc.load(pg + F::VS, th % kKv4Tokens);
+        };
+        bool lost = false;   // a wait gave up: go on without waiting, to the same barriers
+        page_ids(0);
+        read_k(0);
+        read_v(0);
+        for (int st = 0; st < steps; st++) {
+            const uint32_t mask = present_now;
+            if (st + 1 < steps) page_ids(st + 1);
+            if (st && !lost) lost = !wide_wait(kfree, (st - 1) & 1, stop, a.status);
+            if (th == 0) present[st & 1] = mask;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int tok = 32 * w + 8 * k + (lane >> 2);
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const uint32_t sc = b & 1 ? ksc[k].word(b) >> 16 : ksc[k].word(b) & 0xffffu;
+                    const uint32_t two = sc | (sc << 16);
+                    uint4 v;
+                    kv4_word(kw[k][b], two & 0x7ff07ff0u, (two & 0x000f000fu) | 0x64006400u,
+                             ((two << 4) & 0x00f000f0u) | 0xd400d400u, reinterpret_cast<uint32_t*>(&v));
+                    const int ch = 4 * b + (lane & 3);
+                    *reinterpret_cast<uint4*>(sm + C::OFF_K + (ch >> 3) * C::ATOM + tok * 128 +
+                                              (((ch & 7) ^ (tok & 7)) << 4)) = v;
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(kfull);
+            if (st + 1 < steps) read_k(st + 1);
+            // V scales to [page][block][token]
+            uint16_t* vs = reinterpret_cast<uint16_t*>(sm + C::OFF_VS + (st & 1) * C::VS);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+                vs[(th / kKv4Tokens * NB + b) * 16 + th % kKv4Tokens] =
+                    (uint16_t)(b & 1 ? vsc.word(b) >> 16 : vsc.word(b));
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (st && !lost) lost = !wide_wait(vfree, (st - 1) & 1, stop, a.status);
+#pragma unroll
+            for (int k = 0; k < VI; k++) {
+                const int p = vp + k * (kWidePages / VI), b = vm / 2;
+                uint32_t sc[8];   // tokens 2t, 2t + 1
+                lds_words<8>(sc, reinterpret_cast<const uint8_t*>(vs + (p * NB + b) * 16));
+                uint32_t lo[8], hi[8];   // dims 16 vm + vg and + 8, token pairs
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const uint32_t x = vw[k][t], y = x >> 8;
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint32_t q = u ? y : x, s2 = sc[t + 4 * u];
+                        const uint32_t d = s2 & 0x7ff07ff0u;
+                        lo[t + 4 * u] = hmul2u(hsub2u((q & 0x000f000fu) | 0x64006400u,
+                                                      (s2 & 0x000f000fu) | 0x64006400u), d);
+                        hi[t + 4 * u] = hmul2u(hfma2u((q & 0x00f000f0u) | 0x64006400u, 0x2c002c00u,
+                                                      ((s2 << 4) & 0x00f000f0u) | 0xd400d400u), d);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int ch = (p & 3) * 2 + u;
+                    uint8_t* at = sm + C::OFF_V + (p >> 2) * C::VATOM + (16 * vm + vg) * 128 + ((ch ^ vg) << 4);
+                    *reinterpret_cast<uint4*>(at) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+                    *reinterpret_cast<uint4*>(at + 8 * 128) =
+                        make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(vfull);
+            if (st + 1 < steps) read_v(st + 1);
+        }
+    } else if (lane == 0) {
+        // ---- products -------------------------------------------------------------
+        constexpr uint32_t iqk = wide_idesc(128, kWideTok), ipv = wide_idesc(128, HD);
+        const uint32_t qa = smem_u32(sm), ka = smem_u32(sm + C::OFF_K), va = smem_u32(sm + C::OFF_V);
+        auto qk = [&](int x) {
+            const uint32_t d = tmem + x * C::TILE_COLS;
+#pragma unroll 1
+            for (int part = 0; part < 2; part++)
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++) {
+                    const uint64_t qd = sw128_kmajor_desc(qa + ((x * 2 + part) * C::ATOMS + k / 4) * C::ATOM) + 2 * (k & 3);
+                    const uint64_t kd = sw128_kmajor_desc(ka + (k / 4) * C::ATOM) + 2 * (k & 3);
+                    mma_f16_ss(d, qd, kd, iqk, part | k);
+                }
+            tc_commit(sfull + x);
+        };
+        auto pv = [&](int x, int st) {
+            const uint32_t d = tmem + x * C::TILE_COLS + 128;
+#pragma unroll 1
+            for (int part = 0; part < 2; part++)
+#pragma unroll
+                for (int p = 0; p < kWidePages; p++) {
+                    const uint64_t vd = sw128_kmajor_desc(va + (p / 4) * C::VATOM) + 2 * (p & 3);
+                    mma_f16_ts(d, tmem + x * C::TILE_COLS + (p / 2) * 32 + part * 16 + (p & 1) * 8, vd, ipv,
+                               st | part | p);
+                }
+        };
+        bool ok = wide_wait(qfull, 0, stop, a.status) && wide_wait(kfull, 0, stop, a.status);
+        tc_fence_after();
+        if (ok) {
+            for (int x = 0; x < tiles; x++) qk(x);
+            tc_commit(kfree);
+        }
+        for (int st = 0; ok && st < steps; st++) {
+            for (int x = 0; x < tiles; x++) {
+                ok = wide_wait(pfull + x, st & 1, stop, a.status) &&
+                     (x || wide_wait(vfull, st & 1, stop, a.status));
+                if (!ok) break;
+                tc_fence_after();
+                pv(x, st);
+                if (x == tiles - 1) tc_commit(vfree);
+                if (st + 1 < steps) {
+                    if (x == 0 && !(ok = wide_wait(kfull, (st + 1) & 1, stop, a.status))) break;
+                    tc_fence_after();
+                    qk(x);
+                    if (x == tiles - 1) tc_commit(kfree);
+                }
+            }
+        }
+        tc_commit(odone);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        // every product has retired before TMEM is released
+        mbar_wait_bounded(odone, 0, a.status, AXQ8_ERR_WAIT_TIMEOUT);
+        tc_fence_after();
+        tmem_dealloc(tmem, C::TMEM_COLS);
+    }
+}
+
+}  // namespace axq8
