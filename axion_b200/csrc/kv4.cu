@@ -265,6 +265,15 @@ cudaError_t launch_wide(const axkv4_cache_t* c, const float* q, int64_t ldq, int
     const cudaError_t e = cudaFuncSetAttribute(kv4_attn_wide_kernel<HD>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
+    // the roles' register split draws on what the launch has
+    static int regs = 0;
+    if (!regs) {
+        cudaFuncAttributes fa;
+        const cudaError_t e2 = cudaFuncGetAttributes(&fa, kv4_attn_wide_kernel<HD>);
+        if (e2 != cudaSuccess) return e2;
+        regs = fa.numRegs;
+    }
+    if (regs < kWideRegs) return cudaErrorInvalidConfiguration;
     const int64_t rows = (int64_t)std::min(max_rows, n_rows) * a.G;
     return launch_k(kv4_attn_wide_kernel<HD>, dim3((unsigned)((rows + 255) / 256), c->n_kv_heads, chunks),
                     dim3(kWideThreads), smem, s, false, a);

@@ -15,8 +15,8 @@
 // the order in which a code word's nibbles come out in pairs.
 //
 // Roles: warps 0-3 and 4-7 the softmax of tile 0 and 1 (a thread is a row),
-// warps 8-11 form the K and V^T tiles from page words that they read a step
-// ahead, warp 12 issues the products in the order
+// warps 8-11 form the K tiles and 12-15 the V^T tiles from page words that they
+// read a step ahead, warp 16 issues the products in the order
 //   PV(tile 0, step j)  QK(tile 0, j + 1)  PV(tile 1, j)  QK(tile 1, j + 1)
 // so that each tile's softmax runs under the other tile's products.  P takes
 // the place of S in TMEM, 32 tokens at a time.  The softmax reference moves (and
@@ -40,7 +40,10 @@ namespace axq8 {
 
 constexpr int kWideTok = 128;                      // tokens of a step
 constexpr int kWidePages = kWideTok / kKv4Tokens;
-constexpr int kWideThreads = 13 * 32;
+constexpr int kWideThreads = 20 * 32;              // five warpgroups, the last one for the products
+// Registers of a thread by role (setmaxnreg); at launch each has 96.
+constexpr int kWideRegs = 96, kWideRegsSoft = 128, kWideRegsTiles = 80, kWideRegsMma = 64;
+static_assert(2 * kWideRegsSoft + 2 * kWideRegsTiles + kWideRegsMma <= 5 * kWideRegs, "registers of the launch");
 
 struct WideArgs {
     Kv4Pages c;
@@ -66,11 +69,21 @@ struct WideCfg {
     static constexpr int OFF_K = Q, OFF_V = Q + K;
     static constexpr int OFF_VS = OFF_V + V;                // V scales [2][page][block][16]
     static constexpr int VS = kWidePages * (HD / 32) * 32;
-    static constexpr int OFF_BAR = OFF_VS + 2 * VS;
+    static constexpr int OFF_MUL = OFF_VS + 2 * VS;         // score factors of the rows [2][128]
+    static constexpr int OFF_BAR = OFF_MUL + 2 * 128 * 4;
     static constexpr int SMEM = 1024 + OFF_BAR + 256;
     static constexpr int TILE_COLS = 128 + (HD < 32 ? 32 : HD);   // S (P), then O
     static constexpr int TMEM_COLS = 512;
 };
+
+template <int N>
+__device__ __forceinline__ void wide_regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void wide_regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 // Instruction descriptor, kind::f16: D fp32 (bits 4-5 = 1), A and B fp16, both
 // K-major, N >> 3 at bit 17, M >> 4 at bit 24.
@@ -103,6 +116,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
         "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
         "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() {
@@ -188,7 +206,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
         *stop = 0;
         fence_mbar_init();
     }
-    if (warp == 12) tmem_alloc(tmem_slot, C::TMEM_COLS);
+    if (warp == 16) tmem_alloc(tmem_slot, C::TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -196,43 +214,61 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
 
     if (warp < 8) {
         // ---- softmax: thread = row of tile x --------------------------------------
+        wide_regs_inc<kWideRegsSoft>();
         const int x = warp >> 2;
         if (x < tiles) {
-            const int r = (warp & 3) * 32 + lane, m = m0 + 128 * x + r;
-            const bool live = m < rows;
-            const int j = min(m, rows - 1) / a.G, head = kvh * a.G + min(m, rows - 1) - j * a.G;
-            const float* qp = a.q + (int64_t)(r0 + j) * a.ldq + (int64_t)head * HD;
-            float mx = 0.0f;
-            for (int d = 0; d < HD; d += 4) {
-                const float4 v = __ldg(reinterpret_cast<const float4*>(qp + d));
-                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            // Q rows of this warp: the fp32 row into the bytes that its two parts will
+            // take, then row by row into those, LPR lanes (8 dims each) to a row
+            constexpr int LPR = HD / 8, RPI = 32 / LPR, SEG = HD >= 64 ? 8 : 4;   // 16-byte chunks of a segment
+            float* mul_s = reinterpret_cast<float*>(sm + C::OFF_MUL) + x * 128;
+            auto q_raw = [&](int row, int c) {
+                return sm + (x * 2 * C::ATOMS + c / SEG) * C::ATOM + row * 128 + c % SEG * 16;
+            };
+#pragma unroll 4
+            for (int it = 0; it < HD / 4; it++) {
+                const int rr = (warp & 3) * 32 + it * 32 / (HD / 4) + lane / (HD / 4), c = lane % (HD / 4);
+                const int mm = m0 + 128 * x + rr, jj = min(mm, rows - 1) / a.G;
+                cp_async16_zfill(q_raw(rr, c), a.q + (int64_t)(r0 + jj) * a.ldq +
+                                 (int64_t)(kvh * a.G + min(mm, rows - 1) - jj * a.G) * HD + 4 * c, mm < rows);
             }
-            // 2^k with max |q| 2^k in [2^13, 2^14)
-            const int ex = max((int)(__float_as_uint(mx) >> 23), 40) - 127;
-            const float up = live ? __uint_as_float((uint32_t)(127 + 13 - ex) << 23) : 0.0f;
-            const float mul = __uint_as_float((uint32_t)(127 - 13 + ex) << 23) * a.scale;
-            uint8_t* qs = sm + x * 2 * C::ATOMS * C::ATOM;
+            cp_async_wait_all();
+            __syncwarp();
 #pragma unroll 2
-            for (int ch = 0; ch < HD / 8; ch++) {
-                const float4 u = __ldg(reinterpret_cast<const float4*>(qp + 8 * ch));
-                const float4 v = __ldg(reinterpret_cast<const float4*>(qp + 8 * ch + 4));
+            for (int it = 0; it < 32 / RPI; it++) {
+                const int rr = (warp & 3) * 32 + it * RPI + lane / LPR, ch = lane % LPR;
+                const float4 u = *reinterpret_cast<const float4*>(q_raw(rr, 2 * ch));
+                const float4 v = *reinterpret_cast<const float4*>(q_raw(rr, 2 * ch + 1));
+                float mx = fmaxf(fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))),
+                                 fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+#pragma unroll
+                for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                // 2^k with max |q| 2^k in [2^13, 2^14)
+                const int ex = max((int)(__float_as_uint(mx) >> 23), 40) - 127;
+                const float up = __uint_as_float((uint32_t)(127 + 13 - ex) << 23);
+                if (ch == 0) mul_s[rr] = __uint_as_float((uint32_t)(127 - 13 + ex) << 23) * a.scale;
                 uint4 hi, lo;
                 split2(u.x * up, v.x * up, hi.x, lo.x);
                 split2(u.y * up, v.y * up, hi.y, lo.y);
                 split2(u.z * up, v.z * up, hi.z, lo.z);
                 split2(u.w * up, v.w * up, hi.w, lo.w);
-                uint8_t* at = qs + (ch >> 3) * C::ATOM + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                __syncwarp();   // the rows are read
+                uint8_t* at = sm + (x * 2 * C::ATOMS + (ch >> 3)) * C::ATOM + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
                 *reinterpret_cast<uint4*>(at) = hi;
                 *reinterpret_cast<uint4*>(at + C::ATOMS * C::ATOM) = lo;
             }
             fence_async_smem();
+            __syncwarp();
             mbar_arrive(qfull);
 
+            const int r = (warp & 3) * 32 + lane, m = m0 + 128 * x + r;
+            const bool live = m < rows;
+            const int j = min(m, rows - 1) / a.G;
+            const float mul = mul_s[r];
             const int pos = live && seq_ok ? min(pos0 + j, room - 1) : -1;   // the last token seen
             const int sees = __reduce_min_sync(0xffffffffu, live ? pos : 0x7fffffff);
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * C::TILE_COLS, to = ts + 128;
-            float base = -CUDART_INF_F, l = 0.0f;
-            uint32_t s[32];
+            float base = -CUDART_INF_F, l[2] = {0.0f, 0.0f};
+            uint32_t s[2][32];   // 32 tokens each, the next ones on their way
             bool ok = true;
             for (int st = 0; st < steps; st++) {
                 if (!__all_sync(0xffffffffu, wide_wait(sfull + x, st & 1, stop, a.status))) {
@@ -240,58 +276,80 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                     break;
                 }
                 tc_fence_after();
+                tmem_ld32(ts, s[0]);
+                tmem_ld32(ts + 32, s[1]);
                 const int tok0 = st * kWideTok;
                 const uint32_t pages = present[st & 1];
                 const bool whole = tok0 + kWideTok - 1 <= sees && pages == (1u << kWidePages) - 1;
-                auto load = [&](int c) {
-                    tmem_ld32(ts + 32 * c, s);
-                    tmem_wait_ld32(s);
-                    if (!whole) {
+                auto mask = [&](int c, uint32_t* v) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            const int tok = 32 * c + e;
-                            if (tok0 + tok > pos || !((pages >> (tok / kKv4Tokens)) & 1)) s[e] = 0xff800000u;
-                        }
+                    for (int e = 0; e < 32; e++) {
+                        const int tok = 32 * c + e;
+                        if (tok0 + tok > pos || !((pages >> (tok / kKv4Tokens)) & 1)) v[e] = 0xff800000u;
                     }
                 };
-                float top = -CUDART_INF_F;
-#pragma unroll 1
-                for (int c = 0; c < kWideTok / 32; c++) {
-                    load(c);
+                float t4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-                    for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(s[e]));
+                for (int c = 0; c < kWideTok / 32; c += 2) {
+                    tmem_wait_ld32(s[0]);
+                    tmem_wait_ld32(s[1]);
+                    if (!whole) {
+                        mask(c, s[0]);
+                        mask(c + 1, s[1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) t4[e & 3] = fmaxf(t4[e & 3], __uint_as_float(s[0][e]));
+                    if (c == 0) tmem_ld32(ts + 64, s[0]);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) t4[e & 3] = fmaxf(t4[e & 3], __uint_as_float(s[1][e]));
+                    if (c == 0) tmem_ld32(ts + 96, s[1]);
                 }
-                top *= mul;
+                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * mul;
                 const bool over = top > base + 8.0f;
                 if (__any_sync(0xffffffffu, over)) {
                     const float f = over ? ex2(base - top) : 1.0f;   // 0 from -inf
                     if (over) base = top;
-                    l *= f;
+                    l[0] *= f;
+                    l[1] *= f;
                     if (st) {
 #pragma unroll 1
                         for (int c = 0; c < HD / 32; c++) {
-                            tmem_ld32(to + 32 * c, s);
-                            tmem_wait_ld32(s);
+                            uint32_t o[32];
+                            tmem_ld32(to + 32 * c, o);
+                            tmem_wait_ld32(o);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) s[e] = __float_as_uint(__uint_as_float(s[e]) * f);
-                            tmem_st32(to + 32 * c, s);
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st32(to + 32 * c, o);
                         }
                         tmem_wait_st();
                     }
                 }
                 const float b7 = base == -CUDART_INF_F ? 0.0f : base - 7.0f;
-#pragma unroll 1
-                for (int c = 0; c < kWideTok / 32; c++) {
-                    load(c);
-                    uint32_t pw[32];   // columns: 16 high pairs, then 16 residual pairs
+                // the last 64 tokens are still in registers: from there back
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float w0 = ex2(fmaf(__uint_as_float(s[2 * e]), mul, -b7));
-                        const float w1 = ex2(fmaf(__uint_as_float(s[2 * e + 1]), mul, -b7));
-                        l += w0 + w1;
-                        split2(w0, w1, pw[e], pw[16 + e]);
+                for (int k = 0; k < kWideTok / 32; k++) {
+                    constexpr int order[4] = {2, 3, 0, 1};
+                    const int c = order[k];
+                    uint32_t* v = s[c & 1];
+                    if (k >= 2) {
+                        tmem_wait_ld32(v);
+                        if (!whole) mask(c, v);
                     }
-                    tmem_st32(ts + 32 * c, pw);
+#pragma unroll
+                    for (int p = 0; p < 2; p++) {   // 16 tokens: 8 columns of high pairs, 8 of residuals
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float w0 = ex2(fmaf(__uint_as_float(v[16 * p + 2 * e]), mul, -b7));
+                            const float w1 = ex2(fmaf(__uint_as_float(v[16 * p + 2 * e + 1]), mul, -b7));
+                            l[0] += w0;
+                            l[1] += w1;
+                            split2(w0, w1, hi[e], lo[e]);
+                        }
+                        tmem_st8(ts + 32 * c + 8 * p, hi);
+                        tmem_st8(ts + 32 * c + 16 + 8 * p, lo);
+                    }
+                    if (k < 2) tmem_ld32(ts + 32 * order[k + 2], v);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -300,147 +358,172 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
             // O / l
             if (ok && __all_sync(0xffffffffu, wide_wait(odone, 0, stop, a.status))) {
                 tc_fence_after();
-                const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;   // nothing seen: zeros
-                float* op = a.out + (int64_t)(r0 + j) * a.n_heads * HD + (int64_t)head * HD;
+                const float sum = l[0] + l[1];
+                const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;   // nothing seen: zeros
+                float* op = a.out + (int64_t)(r0 + j) * a.n_heads * HD +
+                            (int64_t)(kvh * a.G + min(m, rows - 1) - j * a.G) * HD;
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; c++) {
-                    tmem_ld32(to + 32 * c, s);
-                    tmem_wait_ld32(s);
+                    tmem_ld32(to + 32 * c, s[0]);
+                    tmem_wait_ld32(s[0]);
                     if (live) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
                             *reinterpret_cast<float4*>(op + 32 * c + e) =
-                                make_float4(__uint_as_float(s[e]) * inv, __uint_as_float(s[e + 1]) * inv,
-                                            __uint_as_float(s[e + 2]) * inv, __uint_as_float(s[e + 3]) * inv);
+                                make_float4(__uint_as_float(s[0][e]) * inv, __uint_as_float(s[0][e + 1]) * inv,
+                                            __uint_as_float(s[0][e + 2]) * inv, __uint_as_float(s[0][e + 3]) * inv);
                     }
                 }
             }
         }
-    } else if (warp < 12) {
-        // ---- K and V^T tiles ------------------------------------------------------
-        const int w = warp - 8, th = threadIdx.x - 256;
-        constexpr int VT = HD / 2, VI = HD / 32;           // threads of a page's V, pages of a thread
-        const int vp = th / VT, vm = (th % VT) / 8, vg = th % 8;
+    } else if (warp < 16) {
+        // ---- K tiles (warps 8-11) and V^T tiles (12-15) --------------------------------
+        wide_regs_dec<kWideRegsTiles>();
+        const int w = warp & 3, th = threadIdx.x & 127;
         const int* row = a.c.table + (int64_t)seq * a.c.max_blocks;
-        uint32_t kw[4][NB], vw[VI][4], present_now = 0;
-        Scales<NB> ksc[4], vsc;
+        bool lost = false;   // a wait gave up: go on without waiting, to the same barriers
         int ids = -1;
-        auto page_ids = [&](int st) {      // lane p: page p of step st
+        auto page_ids = [&](int st) {      // lane p: page p of step st; a bit for each that is there
             const int blk = st * kWidePages + (lane & 7);
             const bool in = blk * kKv4Tokens < ctx;
             ids = in ? __ldg(row + blk) : -1;
-            const bool bad = (unsigned)ids >= (unsigned)a.c.n_pages;
-            if (bad) {
-                if (in && lane < 8) record_status(a.status, AXQ8_ERR_INVALID);
+            if ((unsigned)ids >= (unsigned)a.c.n_pages) {
+                if (in && th < 8) record_status(a.status, AXQ8_ERR_INVALID);
                 ids = -1;
             }
-            present_now = __ballot_sync(0xffffffffu, lane < 8 && ids >= 0);
+            return __ballot_sync(0xffffffffu, lane < 8 && ids >= 0);
         };
         auto page_at = [&](int p) {
             const int id = __shfl_sync(0xffffffffu, ids, p);
             return id < 0 ? nullptr : a.c.pages + ((int64_t)id * a.c.n_kv + kvh) * F::BYTES;
         };
-        auto read_k = [&](int st) {        // tokens 32 w + 8 k + lane / 4, chunk lane % 4
+        if (warp < 12) {
+            uint32_t kw[4][NB], there = 0;
+            Scales<NB> ksc[4];
+            auto read_k = [&](int st) {        // tokens 32 w + 8 k + lane / 4, chunk lane % 4
+                there = page_ids(st);
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int tok = 32 * w + 8 * k + (lane >> 2), slot = tok % kKv4Tokens;
-                const uint8_t* pg = page_at(tok / kKv4Tokens);
-                const bool in = pg && st * kWideTok + tok < ctx;
+                for (int k = 0; k < 4; k++) {
+                    const int tok = 32 * w + 8 * k + (lane >> 2), slot = tok % kKv4Tokens;
+                    const uint8_t* pg = page_at(tok / kKv4Tokens);
+                    const bool in = pg && st * kWideTok + tok < ctx;
 #pragma unroll
-                for (int b = 0; b < NB; b++) kw[k][b] = 0;
+                    for (int b = 0; b < NB; b++) kw[k][b] = 0;
 #pragma unroll
-                for (int b = 0; b < Scales<NB>::W; b++) ksc[k].w[b] = 0;
-                if (in) {
-                    lds_words<NB>(kw[k], pg + slot * (HD / 2) + (lane & 3) * (HD / 8));
-                    ksc[k].load(pg + F::KS, slot);
-                }
-            }
-        };
-        auto read_v = [&](int st) {
-#pragma unroll
-            for (int k = 0; k < VI; k++) {
-                const uint8_t* pg = page_at(vp + k * (kWidePages / VI));
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-                    vw[k][t] = pg ? __ldg(reinterpret_cast<const uint32_t*>(
-                                        pg + F::V + (vm / F::TPG) * (128 * F::TPG) + (vg * 4 + t) * (4 * F::TPG) +
-                                        (vm % F::TPG) * 4))
-                                  : 0u;
-            }
-            const uint8_t* pg = page_at(th / kKv4Tokens % kWidePages);
-            // the scales of token th; slots behind the last token hold any bits
-#pragma unroll
-            for (int b = 0; b < Scales<NB>::W; b++) vsc.w[b] = 0;
-            if (pg && st * kWideTok + th < ctx) vsc.load(pg + F::VS, th % kKv4Tokens);
-        };
-        bool lost = false;   // a wait gave up: go on without waiting, to the same barriers
-        page_ids(0);
-        read_k(0);
-        read_v(0);
-        for (int st = 0; st < steps; st++) {
-            const uint32_t mask = present_now;
-            if (st + 1 < steps) page_ids(st + 1);
-            if (st && !lost) lost = !wide_wait(kfree, (st - 1) & 1, stop, a.status);
-            if (th == 0) present[st & 1] = mask;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int tok = 32 * w + 8 * k + (lane >> 2);
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const uint32_t sc = b & 1 ? ksc[k].word(b) >> 16 : ksc[k].word(b) & 0xffffu;
-                    const uint32_t two = sc | (sc << 16);
-                    uint4 v;
-                    kv4_word(kw[k][b], two & 0x7ff07ff0u, (two & 0x000f000fu) | 0x64006400u,
-                             ((two << 4) & 0x00f000f0u) | 0xd400d400u, reinterpret_cast<uint32_t*>(&v));
-                    const int ch = 4 * b + (lane & 3);
-                    *reinterpret_cast<uint4*>(sm + C::OFF_K + (ch >> 3) * C::ATOM + tok * 128 +
-                                              (((ch & 7) ^ (tok & 7)) << 4)) = v;
-                }
-            }
-            fence_async_smem();
-            mbar_arrive(kfull);
-            if (st + 1 < steps) read_k(st + 1);
-            // V scales to [page][block][token]
-            uint16_t* vs = reinterpret_cast<uint16_t*>(sm + C::OFF_VS + (st & 1) * C::VS);
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-                vs[(th / kKv4Tokens * NB + b) * 16 + th % kKv4Tokens] =
-                    (uint16_t)(b & 1 ? vsc.word(b) >> 16 : vsc.word(b));
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (st && !lost) lost = !wide_wait(vfree, (st - 1) & 1, stop, a.status);
-#pragma unroll
-            for (int k = 0; k < VI; k++) {
-                const int p = vp + k * (kWidePages / VI), b = vm / 2;
-                uint32_t sc[8];   // tokens 2t, 2t + 1
-                lds_words<8>(sc, reinterpret_cast<const uint8_t*>(vs + (p * NB + b) * 16));
-                uint32_t lo[8], hi[8];   // dims 16 vm + vg and + 8, token pairs
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const uint32_t x = vw[k][t], y = x >> 8;
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const uint32_t q = u ? y : x, s2 = sc[t + 4 * u];
-                        const uint32_t d = s2 & 0x7ff07ff0u;
-                        lo[t + 4 * u] = hmul2u(hsub2u((q & 0x000f000fu) | 0x64006400u,
-                                                      (s2 & 0x000f000fu) | 0x64006400u), d);
-                        hi[t + 4 * u] = hmul2u(hfma2u((q & 0x00f000f0u) | 0x64006400u, 0x2c002c00u,
-                                                      ((s2 << 4) & 0x00f000f0u) | 0xd400d400u), d);
+                    for (int b = 0; b < Scales<NB>::W; b++) ksc[k].w[b] = 0;
+                    if (in) {
+                        lds_words<NB>(kw[k], pg + slot * (HD / 2) + (lane & 3) * (HD / 8));
+                        ksc[k].load(pg + F::KS, slot);
                     }
                 }
+            };
+            read_k(0);
+            for (int st = 0; st < steps; st++) {
+                // half of the values first, so that little stands between the old tile's last
+                // product and the new tile's first
+                uint4 kv[2][NB];
+                auto form = [&](int k) {
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int ch = (p & 3) * 2 + u;
-                    uint8_t* at = sm + C::OFF_V + (p >> 2) * C::VATOM + (16 * vm + vg) * 128 + ((ch ^ vg) << 4);
-                    *reinterpret_cast<uint4*>(at) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
-                    *reinterpret_cast<uint4*>(at + 8 * 128) =
-                        make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+                    for (int b = 0; b < NB; b++) {
+                        const uint32_t sc = b & 1 ? ksc[k].word(b) >> 16 : ksc[k].word(b) & 0xffffu;
+                        const uint32_t two = sc | (sc << 16);
+                        kv4_word(kw[k][b], two & 0x7ff07ff0u, (two & 0x000f000fu) | 0x64006400u,
+                                 ((two << 4) & 0x00f000f0u) | 0xd400d400u, reinterpret_cast<uint32_t*>(&kv[k & 1][b]));
+                    }
+                };
+                auto store = [&](int k) {
+                    const int tok = 32 * w + 8 * k + (lane >> 2);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const int ch = 4 * b + (lane & 3);
+                        *reinterpret_cast<uint4*>(sm + C::OFF_K + (ch >> 3) * C::ATOM + tok * 128 +
+                                                  (((ch & 7) ^ (tok & 7)) << 4)) = kv[k & 1][b];
+                    }
+                };
+                form(0);
+                form(1);
+                if (st && !lost) lost = !wide_wait(kfree, (st - 1) & 1, stop, a.status);
+                if (th == 0) present[st & 1] = there;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    store(k);
+                    if (k < 2) form(k + 2);
                 }
+                fence_async_smem();
+                mbar_arrive(kfull);
+                __syncwarp();
+                if (st + 1 < steps) read_k(st + 1);
             }
-            fence_async_smem();
-            mbar_arrive(vfull);
-            if (st + 1 < steps) read_v(st + 1);
+        } else {
+            constexpr int VT = HD / 2, VI = HD / 32;           // threads of a page, pages of a thread
+            const int vp = th / VT, vm = (th % VT) / 8, vg = th % 8;
+            uint32_t vw[VI][4];
+            Scales<NB> vsc;
+            auto read_v = [&](int st) {
+                page_ids(st);
+#pragma unroll
+                for (int k = 0; k < VI; k++) {
+                    const uint8_t* pg = page_at(vp + k * (kWidePages / VI));
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        vw[k][t] = pg ? __ldg(reinterpret_cast<const uint32_t*>(
+                                            pg + F::V + (vm / F::TPG) * (128 * F::TPG) + (vg * 4 + t) * (4 * F::TPG) +
+                                            (vm % F::TPG) * 4))
+                                      : 0u;
+                }
+                // the scales of token th; slots behind the last token hold any bits
+                const uint8_t* pg = page_at(th / kKv4Tokens);
+#pragma unroll
+                for (int b = 0; b < Scales<NB>::W; b++) vsc.w[b] = 0;
+                if (pg && st * kWideTok + th < ctx) vsc.load(pg + F::VS, th % kKv4Tokens);
+            };
+            read_v(0);
+            for (int st = 0; st < steps; st++) {
+                // scales to [page][block][token]
+                uint16_t* vs = reinterpret_cast<uint16_t*>(sm + C::OFF_VS + (st & 1) * C::VS);
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                    vs[(th / kKv4Tokens * NB + b) * 16 + th % kKv4Tokens] =
+                        (uint16_t)(b & 1 ? vsc.word(b) >> 16 : vsc.word(b));
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (st && !lost) lost = !wide_wait(vfree, (st - 1) & 1, stop, a.status);
+#pragma unroll
+                for (int k = 0; k < VI; k++) {
+                    const int p = vp + k * (kWidePages / VI), b = vm / 2;
+                    uint32_t sc[8];   // tokens 2t, 2t + 1
+                    lds_words<8>(sc, reinterpret_cast<const uint8_t*>(vs + (p * NB + b) * 16));
+                    uint32_t lo[8], hi[8];   // dims 16 vm + vg and + 8, token pairs
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        const uint32_t x = vw[k][t], y = x >> 8;
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t q = u ? y : x, s2 = sc[t + 4 * u];
+                            const uint32_t d = s2 & 0x7ff07ff0u;
+                            lo[t + 4 * u] = hmul2u(hsub2u((q & 0x000f000fu) | 0x64006400u,
+                                                          (s2 & 0x000f000fu) | 0x64006400u), d);
+                            hi[t + 4 * u] = hmul2u(hfma2u((q & 0x00f000f0u) | 0x64006400u, 0x2c002c00u,
+                                                          ((s2 << 4) & 0x00f000f0u) | 0xd400d400u), d);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const int ch = (p & 3) * 2 + u;
+                        uint8_t* at = sm + C::OFF_V + (p >> 2) * C::VATOM + (16 * vm + vg) * 128 + ((ch ^ vg) << 4);
+                        *reinterpret_cast<uint4*>(at) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+                        *reinterpret_cast<uint4*>(at + 8 * 128) =
+                            make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+                    }
+                }
+                fence_async_smem();
+                mbar_arrive(vfull);
+                __syncwarp();
+                if (st + 1 < steps) read_v(st + 1);
+            }
         }
-    } else if (lane == 0) {
+    } else {
+      wide_regs_dec<kWideRegsMma>();
+      if (warp == 16 && lane == 0) {
         // ---- products -------------------------------------------------------------
         constexpr uint32_t iqk = wide_idesc(128, kWideTok), ipv = wide_idesc(128, HD);
         const uint32_t qa = smem_u32(sm), ka = smem_u32(sm + C::OFF_K), va = smem_u32(sm + C::OFF_V);
@@ -490,10 +573,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
             }
         }
         tc_commit(odone);
+      }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         // every product has retired before TMEM is released
         mbar_wait_bounded(odone, 0, a.status, AXQ8_ERR_WAIT_TIMEOUT);
         tc_fence_after();
