@@ -19,8 +19,10 @@
 // read a step ahead, warp 16 issues the products in the order
 //   PV(tile 0, step j)  QK(tile 0, j + 1)  PV(tile 1, j)  QK(tile 1, j + 1)
 // so that each tile's softmax runs under the other tile's products.  P takes
-// the place of S in TMEM, 32 tokens at a time.  The softmax reference moves (and
-// O is rescaled) only when a score exceeds it by more than 8 (base 2).
+// the place of S in TMEM, 32 tokens at a time, in one pass: the softmax
+// reference (base 2, a whole number) moves only when a score exceeds it by more
+// than 8, and then O and the step's earlier P are multiplied by a power of two.
+// O rows go out through shared memory.
 //
 // Bound: 4 x 128 x 128 x HD multiply-adds a step and tile.  Every wait is
 // bounded; a role that gives up raises a flag, and all stop.
@@ -72,6 +74,8 @@ struct WideCfg {
     static constexpr int OFF_MUL = OFF_VS + 2 * VS;         // score factors of the rows [2][128]
     static constexpr int OFF_BAR = OFF_MUL + 2 * 128 * 4;
     static constexpr int SMEM = 1024 + OFF_BAR + 256;
+    static constexpr int OROW = HD * 4 + 16;                // bytes of an output row on its way out
+    static_assert(256 * OROW <= OFF_VS, "output rows");
     static constexpr int TILE_COLS = 128 + (HD < 32 ? 32 : HD);   // S (P), then O
     static constexpr int TMEM_COLS = 512;
 };
@@ -106,21 +110,35 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
-        "%29, %30, %31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
                  : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+        "%13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() {
@@ -157,6 +175,33 @@ __device__ __forceinline__ bool wide_wait(uint64_t* bar, uint32_t parity, volati
     return false;
 }
 
+// The softmax reference has moved: n16 times 16 columns of O (fp32) times f, and
+// `pages` 16-token pieces of P (fp16 pairs) times 2^down.
+__device__ __noinline__ void wide_rescale(int n16, uint32_t o, int pages, uint32_t ts, int down, float f) {
+    uint32_t v[16];
+    tmem_wait_st();   // P as written so far
+#pragma unroll 1
+    for (int c = 0; c < n16; c++) {
+        tmem_ld16(o + 16 * c, v);
+        tmem_wait_ld16(v);
+#pragma unroll
+        for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+        tmem_st16(o + 16 * c, v);
+    }
+#pragma unroll 1
+    for (int p = 0; p < pages; p++) {
+        tmem_ld16(ts + 16 * p, v);
+        tmem_wait_ld16(v);
+        for (int k = down; k < 0; k += 14) {   // fp16 factors go down to 2^-14
+            const uint32_t h = f16_pow2(max(k, -14));
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[e] = hmul2u(v[e], h);
+        }
+        tmem_st16(ts + 16 * p, v);
+    }
+    tmem_wait_st();
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __grid_constant__ WideArgs a) {
     using F = Kv4<HD>;
@@ -166,8 +211,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wide_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
     uint64_t *kfull = bars, *vfull = bars + 1, *kfree = bars + 2, *vfree = bars + 3, *qfull = bars + 4,
-             *sfull = bars + 5, *pfull = bars + 7, *odone = bars + 9;   // sfull, pfull: [tile]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 10);
+             *sfull = bars + 5, *pfull = bars + 7, *odone = bars + 9;   // sfull, pfull, odone: [tile]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
     volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(tmem_slot + 2);   // [2] pages of a step
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -201,8 +246,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
         for (int x = 0; x < 2; x++) {
             mbar_init(sfull + x, 1);
             mbar_init(pfull + x, 128);
+            mbar_init(odone + x, 1);
         }
-        mbar_init(odone, 1);
         *stop = 0;
         fence_mbar_init();
     }
@@ -217,124 +262,94 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
         wide_regs_inc<kWideRegsSoft>();
         const int x = warp >> 2;
         if (x < tiles) {
-            // Q rows of this warp: the fp32 row into the bytes that its two parts will
-            // take, then row by row into those, LPR lanes (8 dims each) to a row
-            constexpr int LPR = HD / 8, RPI = 32 / LPR, SEG = HD >= 64 ? 8 : 4;   // 16-byte chunks of a segment
+            // Q rows of this warp, LPR lanes (8 dims each) to a row, as many rows on their
+            // way as registers hold
+            constexpr int LPR = HD / 8, RPI = 32 / LPR, ITS = 32 / RPI, AHEAD = ITS < 8 ? ITS : 8;
             float* mul_s = reinterpret_cast<float*>(sm + C::OFF_MUL) + x * 128;
-            auto q_raw = [&](int row, int c) {
-                return sm + (x * 2 * C::ATOMS + c / SEG) * C::ATOM + row * 128 + c % SEG * 16;
-            };
-#pragma unroll 4
-            for (int it = 0; it < HD / 4; it++) {
-                const int rr = (warp & 3) * 32 + it * 32 / (HD / 4) + lane / (HD / 4), c = lane % (HD / 4);
-                const int mm = m0 + 128 * x + rr, jj = min(mm, rows - 1) / a.G;
-                cp_async16_zfill(q_raw(rr, c), a.q + (int64_t)(r0 + jj) * a.ldq +
-                                 (int64_t)(kvh * a.G + min(mm, rows - 1) - jj * a.G) * HD + 4 * c, mm < rows);
-            }
-            cp_async_wait_all();
-            __syncwarp();
-#pragma unroll 2
-            for (int it = 0; it < 32 / RPI; it++) {
-                const int rr = (warp & 3) * 32 + it * RPI + lane / LPR, ch = lane % LPR;
-                const float4 u = *reinterpret_cast<const float4*>(q_raw(rr, 2 * ch));
-                const float4 v = *reinterpret_cast<const float4*>(q_raw(rr, 2 * ch + 1));
-                float mx = fmaxf(fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))),
-                                 fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            const int r = (warp & 3) * 32 + lane, m = m0 + 128 * x + r;   // this thread's row
+            const bool live = m < rows;
+            const int j = min(m, rows - 1) / a.G;
+            const int64_t mine = (int64_t)(r0 + j) * a.ldq + (int64_t)(kvh * a.G + min(m, rows - 1) - j * a.G) * HD;
+            const int ch = lane % LPR;
+#pragma unroll 1
+            for (int i0 = 0; i0 < ITS; i0 += AHEAD) {
+                float4 u[AHEAD], v[AHEAD];
 #pragma unroll
-                for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                // 2^k with max |q| 2^k in [2^13, 2^14)
-                const int ex = max((int)(__float_as_uint(mx) >> 23), 40) - 127;
-                const float up = __uint_as_float((uint32_t)(127 + 13 - ex) << 23);
-                if (ch == 0) mul_s[rr] = __uint_as_float((uint32_t)(127 - 13 + ex) << 23) * a.scale;
-                uint4 hi, lo;
-                split2(u.x * up, v.x * up, hi.x, lo.x);
-                split2(u.y * up, v.y * up, hi.y, lo.y);
-                split2(u.z * up, v.z * up, hi.z, lo.z);
-                split2(u.w * up, v.w * up, hi.w, lo.w);
-                __syncwarp();   // the rows are read
-                uint8_t* at = sm + (x * 2 * C::ATOMS + (ch >> 3)) * C::ATOM + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
-                *reinterpret_cast<uint4*>(at) = hi;
-                *reinterpret_cast<uint4*>(at + C::ATOMS * C::ATOM) = lo;
+                for (int k = 0; k < AHEAD; k++) {
+                    const float* qp = a.q + __shfl_sync(0xffffffffu, mine, (i0 + k) * RPI + lane / LPR) + 8 * ch;
+                    u[k] = __ldg(reinterpret_cast<const float4*>(qp));
+                    v[k] = __ldg(reinterpret_cast<const float4*>(qp + 4));
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; k++) {
+                    const int rr = (warp & 3) * 32 + (i0 + k) * RPI + lane / LPR;
+                    float mx = fmaxf(fmaxf(fmaxf(fabsf(u[k].x), fabsf(u[k].y)), fmaxf(fabsf(u[k].z), fabsf(u[k].w))),
+                                     fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
+#pragma unroll
+                    for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    // 2^k with max |q| 2^k in [2^13, 2^14); rows behind the last are zero
+                    const int ex = max((int)(__float_as_uint(mx) >> 23), 40) - 127;
+                    const float up = m0 + 128 * x + rr < rows ? __uint_as_float((uint32_t)(127 + 13 - ex) << 23) : 0.0f;
+                    if (ch == 0) mul_s[rr] = __uint_as_float((uint32_t)(127 - 13 + ex) << 23) * a.scale;
+                    uint4 hi, lo;
+                    split2(u[k].x * up, v[k].x * up, hi.x, lo.x);
+                    split2(u[k].y * up, v[k].y * up, hi.y, lo.y);
+                    split2(u[k].z * up, v[k].z * up, hi.z, lo.z);
+                    split2(u[k].w * up, v[k].w * up, hi.w, lo.w);
+                    uint8_t* at = sm + (x * 2 * C::ATOMS + (ch >> 3)) * C::ATOM + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
+                    *reinterpret_cast<uint4*>(at) = hi;
+                    *reinterpret_cast<uint4*>(at + C::ATOMS * C::ATOM) = lo;
+                }
             }
+            bool lost = false;   // a wait gave up: go on without waiting
             fence_async_smem();
             __syncwarp();
             mbar_arrive(qfull);
 
-            const int r = (warp & 3) * 32 + lane, m = m0 + 128 * x + r;
-            const bool live = m < rows;
-            const int j = min(m, rows - 1) / a.G;
             const float mul = mul_s[r];
             const int pos = live && seq_ok ? min(pos0 + j, room - 1) : -1;   // the last token seen
             const int sees = __reduce_min_sync(0xffffffffu, live ? pos : 0x7fffffff);
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * C::TILE_COLS, to = ts + 128;
             float base = -CUDART_INF_F, l[2] = {0.0f, 0.0f};
             uint32_t s[2][32];   // 32 tokens each, the next ones on their way
-            bool ok = true;
             for (int st = 0; st < steps; st++) {
-                if (!__all_sync(0xffffffffu, wide_wait(sfull + x, st & 1, stop, a.status))) {
-                    ok = false;
-                    break;
-                }
+                if (!lost) lost = !wide_wait(sfull + x, st & 1, stop, a.status);
+                __syncwarp();
                 tc_fence_after();
                 tmem_ld32(ts, s[0]);
-                tmem_ld32(ts + 32, s[1]);
                 const int tok0 = st * kWideTok;
                 const uint32_t pages = present[st & 1];
                 const bool whole = tok0 + kWideTok - 1 <= sees && pages == (1u << kWidePages) - 1;
-                auto mask = [&](int c, uint32_t* v) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const int tok = 32 * c + e;
-                        if (tok0 + tok > pos || !((pages >> (tok / kKv4Tokens)) & 1)) v[e] = 0xff800000u;
-                    }
-                };
-                float t4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-                for (int c = 0; c < kWideTok / 32; c += 2) {
-                    tmem_wait_ld32(s[0]);
-                    tmem_wait_ld32(s[1]);
-                    if (!whole) {
-                        mask(c, s[0]);
-                        mask(c + 1, s[1]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e++) t4[e & 3] = fmaxf(t4[e & 3], __uint_as_float(s[0][e]));
-                    if (c == 0) tmem_ld32(ts + 64, s[0]);
-#pragma unroll
-                    for (int e = 0; e < 32; e++) t4[e & 3] = fmaxf(t4[e & 3], __uint_as_float(s[1][e]));
-                    if (c == 0) tmem_ld32(ts + 96, s[1]);
-                }
-                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * mul;
-                const bool over = top > base + 8.0f;
-                if (__any_sync(0xffffffffu, over)) {
-                    const float f = over ? ex2(base - top) : 1.0f;   // 0 from -inf
-                    if (over) base = top;
-                    l[0] *= f;
-                    l[1] *= f;
-                    if (st) {
-#pragma unroll 1
-                        for (int c = 0; c < HD / 32; c++) {
-                            uint32_t o[32];
-                            tmem_ld32(to + 32 * c, o);
-                            tmem_wait_ld32(o);
-#pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st32(to + 32 * c, o);
-                        }
-                        tmem_wait_st();
-                    }
-                }
-                const float b7 = base == -CUDART_INF_F ? 0.0f : base - 7.0f;
-                // the last 64 tokens are still in registers: from there back
-#pragma unroll
-                for (int k = 0; k < kWideTok / 32; k++) {
-                    constexpr int order[4] = {2, 3, 0, 1};
-                    const int c = order[k];
+                for (int c = 0; c < kWideTok / 32; c++) {
                     uint32_t* v = s[c & 1];
-                    if (k >= 2) {
-                        tmem_wait_ld32(v);
-                        if (!whole) mask(c, v);
+                    tmem_wait_ld32(v);
+                    if (c + 1 < kWideTok / 32) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            const int tok = 32 * c + e;
+                            if (tok0 + tok > pos || !((pages >> (tok / kKv4Tokens)) & 1)) v[e] = 0xff800000u;
+                        }
                     }
+                    float t4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+                    for (int e = 0; e < 32; e++) t4[e & 3] = fmaxf(t4[e & 3], __uint_as_float(v[e]));
+                    const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * mul;
+                    const bool over = top > base + 8.0f;
+                    if (__any_sync(0xffffffffu, over)) {
+                        const float to_base = over ? ceilf(top) : base;
+                        // the factor 2^down; nothing so far: any
+                        const int down = over && base != -CUDART_INF_F ? (int)fmaxf(base - to_base, -120.0f) : 0;
+                        base = to_base;
+                        const float f = __uint_as_float((uint32_t)(127 + down) << 23);
+                        l[0] *= f;
+                        l[1] *= f;
+                        // what is on its way has to arrive before its registers can be moved
+                        if (c + 1 < kWideTok / 32) tmem_wait_ld32(s[(c + 1) & 1]);
+                        if (st || c) wide_rescale(st ? HD / 16 : 0, to, 2 * c, ts, down, f);
+                    }
+                    const float b7 = base == -CUDART_INF_F ? 0.0f : base - 7.0f;
 #pragma unroll
                     for (int p = 0; p < 2; p++) {   // 16 tokens: 8 columns of high pairs, 8 of residuals
                         uint32_t hi[8], lo[8];
@@ -349,31 +364,39 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                         tmem_st8(ts + 32 * c + 8 * p, hi);
                         tmem_st8(ts + 32 * c + 16 + 8 * p, lo);
                     }
-                    if (k < 2) tmem_ld32(ts + 32 * order[k + 2], v);
                 }
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(pfull + x);
             }
-            // O / l
-            if (ok && __all_sync(0xffffffffu, wide_wait(odone, 0, stop, a.status))) {
-                tc_fence_after();
-                const float sum = l[0] + l[1];
-                const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;   // nothing seen: zeros
-                float* op = a.out + (int64_t)(r0 + j) * a.n_heads * HD +
-                            (int64_t)(kvh * a.G + min(m, rows - 1) - j * a.G) * HD;
-#pragma unroll 1
-                for (int c = 0; c < HD / 32; c++) {
-                    tmem_ld32(to + 32 * c, s[0]);
-                    tmem_wait_ld32(s[0]);
-                    if (live) {
+            // O / l: the tile's rows to shared memory (Q and K are read), from there to `out`
+            if (!lost) lost = !wide_wait(odone + x, 0, stop, a.status);
+            __syncwarp();
+            tc_fence_after();
+            const float sum = l[0] + l[1];
+            const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;   // nothing seen: zeros
+            uint8_t* orow = sm + (128 * x + r) * C::OROW;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<float4*>(op + 32 * c + e) =
-                                make_float4(__uint_as_float(s[0][e]) * inv, __uint_as_float(s[0][e + 1]) * inv,
-                                            __uint_as_float(s[0][e + 2]) * inv, __uint_as_float(s[0][e + 3]) * inv);
-                    }
-                }
+            for (int c = 0; c < HD / 32; c++) {
+                tmem_ld32(to + 32 * c, s[0]);
+                tmem_wait_ld32(s[0]);
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<float4*>(orow + (32 * c + e) * 4) =
+                        make_float4(__uint_as_float(s[0][e]) * inv, __uint_as_float(s[0][e + 1]) * inv,
+                                    __uint_as_float(s[0][e + 2]) * inv, __uint_as_float(s[0][e + 3]) * inv);
+            }
+            __syncwarp();
+            // this warp's rows, HD / 4 lanes to a row
+            constexpr int OL = HD / 4;
+            const int64_t oat = (int64_t)(r0 + j) * a.n_heads * HD + (int64_t)(kvh * a.G + min(m, rows - 1) - j * a.G) * HD;
+#pragma unroll 4
+            for (int k = 0; k < OL; k++) {
+                const int rr = k * (32 / OL) + lane / OL;
+                const int64_t at = __shfl_sync(0xffffffffu, oat, rr);
+                if (m0 + 128 * x + (warp & 3) * 32 + rr < rows)
+                    *reinterpret_cast<float4*>(a.out + at + 4 * (lane % OL)) = *reinterpret_cast<const float4*>(
+                        sm + (128 * x + (warp & 3) * 32 + rr) * C::OROW + 16 * (lane % OL));
             }
         }
     } else if (warp < 16) {
@@ -557,13 +580,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
             tc_commit(kfree);
         }
         for (int st = 0; ok && st < steps; st++) {
-            for (int x = 0; x < tiles; x++) {
+            for (int x = 0; x < tiles; x++) {   // tile 1's last product ends last
                 ok = wide_wait(pfull + x, st & 1, stop, a.status) &&
                      (x || wide_wait(vfull, st & 1, stop, a.status));
                 if (!ok) break;
                 tc_fence_after();
                 pv(x, st);
                 if (x == tiles - 1) tc_commit(vfree);
+                else if (st + 1 == steps) tc_commit(odone);
                 if (st + 1 < steps) {
                     if (x == 0 && !(ok = wide_wait(kfull, (st + 1) & 1, stop, a.status))) break;
                     tc_fence_after();
@@ -572,14 +596,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                 }
             }
         }
-        tc_commit(odone);
+        tc_commit(odone + tiles - 1);
       }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 16) {
         // every product has retired before TMEM is released
-        mbar_wait_bounded(odone, 0, a.status, AXQ8_ERR_WAIT_TIMEOUT);
+        mbar_wait_bounded(odone + tiles - 1, 0, a.status, AXQ8_ERR_WAIT_TIMEOUT);
         tc_fence_after();
         tmem_dealloc(tmem, C::TMEM_COLS);
     }
