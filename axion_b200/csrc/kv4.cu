@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "axkv.h"
@@ -201,13 +202,16 @@ NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int entries, int
 }
 
 template <int HD, int COLS>
-cudaError_t launch_narrow_cols(const NarrowArgs& a, int ctas, cudaStream_t s) {
+cudaError_t launch_narrow_cols(DeviceState* ds, const NarrowArgs& a, int ctas, cudaStream_t s) {
     static_assert(NarrowCfg<HD, COLS>::CTAS == (COLS == 4 ? 4 : COLS == 8 ? 3 : 2), "narrow_plan");
     constexpr size_t smem = NarrowCfg<HD, COLS>::SMEM;
     auto kern = kv4_attn_narrow_kernel<HD, COLS>;
-    if (smem > 48 * 1024) {
+    static std::atomic<int> configured[64] = {};   // by device
+    const int dev = ds->device < 64 ? ds->device : 63;
+    if (smem > 48 * 1024 && (dev == 63 || !configured[dev])) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
+        configured[dev] = 1;
     }
     const cudaError_t e = launch_k(kern, dim3(ctas), dim3(kNarrowWarps * 32), smem, s, false, a);
     if (e != cudaSuccess) return e;
@@ -216,10 +220,9 @@ cudaError_t launch_narrow_cols(const NarrowArgs& a, int ctas, cudaStream_t s) {
 }
 
 template <int HD>
-cudaError_t launch_narrow(const NarrowPlan& p, const axkv4_cache_t* c, const float* q, int64_t ldq,
+cudaError_t launch_narrow(DeviceState* ds, const NarrowPlan& p, const axkv4_cache_t* c, const float* q, int64_t ldq,
                           int n_rows, int chunks, int max_rows, int n_heads, const int* q_seq,
-                          const int* q_start, const int* q_pos, float* out, void* ws, int* status,
-                          cudaStream_t s) {
+                          const int* q_start, const int* q_pos, float* out, void* ws, cudaStream_t s) {
     NarrowArgs a = {};
     a.c = pages_of(c);
     a.q = q;
@@ -237,16 +240,16 @@ cudaError_t launch_narrow(const NarrowPlan& p, const axkv4_cache_t* c, const flo
     a.out = out;
     a.split = static_cast<NarrowPart*>(ws);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.records);
-    a.status = status;
-    return p.cols == 4   ? launch_narrow_cols<HD, 4>(a, p.ctas, s)
-           : p.cols == 8 ? launch_narrow_cols<HD, 8>(a, p.ctas, s)
-                         : launch_narrow_cols<HD, 16>(a, p.ctas, s);
+    a.status = ds->status;
+    return p.cols == 4   ? launch_narrow_cols<HD, 4>(ds, a, p.ctas, s)
+           : p.cols == 8 ? launch_narrow_cols<HD, 8>(ds, a, p.ctas, s)
+                         : launch_narrow_cols<HD, 16>(ds, a, p.ctas, s);
 }
 
 template <int HD>
-cudaError_t launch_wide(const axkv4_cache_t* c, const float* q, int64_t ldq, int n_rows, int chunks,
+cudaError_t launch_wide(DeviceState* ds, const axkv4_cache_t* c, const float* q, int64_t ldq, int n_rows, int chunks,
                         int max_rows, int n_heads, const int* q_seq, const int* q_start,
-                        const int* q_pos, float* out, int* status, cudaStream_t s) {
+                        const int* q_pos, float* out, cudaStream_t s) {
     WideArgs a = {};
     a.c = pages_of(c);
     a.q = q;
@@ -260,20 +263,21 @@ cudaError_t launch_wide(const axkv4_cache_t* c, const float* q, int64_t ldq, int
     a.q_pos = q_pos;
     a.scale = 1.4426950408889634f / std::sqrt((float)HD);
     a.out = out;
-    a.status = status;
+    a.status = ds->status;
     constexpr size_t smem = WideCfg<HD>::SMEM;
-    const cudaError_t e = cudaFuncSetAttribute(kv4_attn_wide_kernel<HD>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    // the roles' register split draws on what the launch has
-    static int regs = 0;
-    if (!regs) {
+    static std::atomic<int> configured[64] = {};   // by device
+    const int dev = ds->device < 64 ? ds->device : 63;
+    if (dev == 63 || !configured[dev]) {
+        // the roles' register split draws on what the launch has
         cudaFuncAttributes fa;
-        const cudaError_t e2 = cudaFuncGetAttributes(&fa, kv4_attn_wide_kernel<HD>);
-        if (e2 != cudaSuccess) return e2;
-        regs = fa.numRegs;
+        cudaError_t e = cudaFuncGetAttributes(&fa, kv4_attn_wide_kernel<HD>);
+        if (e == cudaSuccess && fa.numRegs < kWideRegs) e = cudaErrorInvalidConfiguration;
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kv4_attn_wide_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)smem);
+        if (e != cudaSuccess) return e;
+        configured[dev] = 1;
     }
-    if (regs < kWideRegs) return cudaErrorInvalidConfiguration;
     const int64_t rows = (int64_t)std::min(max_rows, n_rows) * a.G;
     return launch_k(kv4_attn_wide_kernel<HD>, dim3((unsigned)((rows + 255) / 256), c->n_kv_heads, chunks),
                     dim3(kWideThreads), smem, s, false, a);
@@ -346,9 +350,8 @@ int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32
     if (workspace_bytes < p.workspace)
         return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: workspace %lld B < %lld B",
                     (long long)workspace_bytes, (long long)p.workspace);
-    AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_narrow, p, c, q, ldq, n_rows, n_rows, 1, n_heads,
-                                  q_seq, nullptr, q_pos, out, workspace, ds->status,
-                                  static_cast<cudaStream_t>(stream)),
+    AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_narrow, ds, p, c, q, ldq, n_rows, n_rows, 1, n_heads,
+                                  q_seq, nullptr, q_pos, out, workspace, static_cast<cudaStream_t>(stream)),
                   "axkv4_decode_attn launch");
     return AXQ8_OK;
 }
@@ -385,8 +388,8 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
     if (!ds) return AXQ8_ERR_CUDA;
     if ((int64_t)max_rows * (n_heads / c->n_kv_heads) >= kWideCols) {
         if (c->n_kv_heads > 65535) return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d KV heads", c->n_kv_heads);
-        AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_wide, c, q, ldq, n_rows, n_chunks, max_rows, n_heads,
-                                      q_seq, q_start, q_pos, out, ds->status,
+        AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_wide, ds, c, q, ldq, n_rows, n_chunks, max_rows, n_heads,
+                                      q_seq, q_start, q_pos, out,
                                       static_cast<cudaStream_t>(stream)),
                       "axkv4_chunk_attn launch");
         return AXQ8_OK;
@@ -398,8 +401,8 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
     if (workspace_bytes < p.workspace)
         return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: workspace %lld B < %lld B",
                     (long long)workspace_bytes, (long long)p.workspace);
-    AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_narrow, p, c, q, ldq, n_rows, n_chunks, max_rows,
-                                  n_heads, q_seq, q_start, q_pos, out, workspace, ds->status,
+    AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_narrow, ds, p, c, q, ldq, n_rows, n_chunks, max_rows,
+                                  n_heads, q_seq, q_start, q_pos, out, workspace,
                                   static_cast<cudaStream_t>(stream)),
                   "axkv4_chunk_attn launch");
     return AXQ8_OK;

@@ -16,12 +16,12 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import check
-from .paged_kv import _on
+from .paged_kv import _DeviceCalls
 
 
-class KVPages:
+class KVPages(_DeviceCalls):
     page_size = 16
+    _what = "KVPages"
 
     def __init__(self, pools: list[torch.Tensor], block_table: torch.Tensor,
                  ref_count: torch.Tensor):
@@ -56,7 +56,10 @@ class KVPages:
                                    self._ptrs.data_ptr(), size, len(pools), self.max_seqs,
                                    self.max_blocks, n_pages)
         self._ref = C.byref(self.c)
+        self._set_device(block_table)
+        self._ws: dict[int, torch.Tensor] = {}
         self._lib = _lib.load()
+        self._need = self._lib.axkv_pages_workspace(self._ref, 0)
 
     @classmethod
     def empty(cls, pools: list[torch.Tensor], max_seqs: int, max_blocks: int) -> "KVPages":
@@ -67,56 +70,40 @@ class KVPages:
         return cls(pools, torch.full((max_seqs, max_blocks), -1, dtype=torch.int32, device=dev),
                    torch.zeros(pools[0].shape[0], dtype=torch.int32, device=dev))
 
-    def _ints(self, what: str, *ts: torch.Tensor) -> list[int]:
+    def _list(self, *ts: torch.Tensor) -> tuple[int, list[int]]:
+        """The common length of request tensors, and their addresses."""
         n = ts[0].shape[0] if ts[0].dim() == 1 else -1
-        for t in ts:
-            if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n \
-                    or t.device != self.block_table.device or not t.is_contiguous():
-                raise RuntimeError(f"KVPages: {what} must be contiguous int32 tensors of one length "
-                                   "on the table's device")
-        return [t.data_ptr() for t in ts]
+        return n, [self._ints(t, n, "requests") for t in ts]
 
     def _workspace(self, n: int) -> torch.Tensor:
-        need = self._lib.axkv_pages_workspace(self._ref, n)
-        return torch.empty(need, dtype=torch.uint8, device=self.block_table.device)
-
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.block_table.device).cuda_stream
+        return self._scratch(self._need + 4 * n)
 
     def reserve(self, seqs: torch.Tensor, tokens: torch.Tensor) -> None:
         """Pages for tokens[i] tokens of sequence seqs[i] (each named once)."""
-        s, t = self._ints("seqs and tokens", seqs, tokens)
-        with _on(self.block_table.device):
-            ws = self._workspace(seqs.shape[0])
-            check(self._lib.axkv_pages_reserve(self._ref, s, t, seqs.shape[0], ws.data_ptr(),
-                                               ws.numel(), self._stream()))
+        n, at = self._list(seqs, tokens)
+        ws = self._workspace(n)
+        self._call(self._lib.axkv_pages_reserve, *at, n, ws.data_ptr(), ws.numel())
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor, tokens: torch.Tensor) -> None:
         """Empty sequence children[i] becomes a copy of the first tokens[i]
         tokens of parents[i]: full pages shared, a partly filled one copied."""
-        a, b, t = self._ints("parents, children and tokens", parents, children, tokens)
-        with _on(self.block_table.device):
-            ws = self._workspace(parents.shape[0])
-            check(self._lib.axkv_pages_fork(self._ref, a, b, t, parents.shape[0], ws.data_ptr(),
-                                            ws.numel(), self._stream()))
+        n, at = self._list(parents, children, tokens)
+        ws = self._workspace(n)
+        self._call(self._lib.axkv_pages_fork, *at, n, ws.data_ptr(), ws.numel())
 
     def free(self, seqs: torch.Tensor) -> None:
         """Sequences give their pages up."""
-        s, = self._ints("seqs", seqs)
-        with _on(self.block_table.device):
-            check(self._lib.axkv_pages_free(self._ref, s, seqs.shape[0], self._stream()))
+        n, at = self._list(seqs)
+        self._call(self._lib.axkv_pages_free, *at, n)
 
     def compact(self) -> torch.Tensor:
         """Live pages to the front of every pool; their number (int32 [1])."""
-        with _on(self.block_table.device):
-            n = torch.empty(1, dtype=torch.int32, device=self.block_table.device)
-            ws = self._workspace(0)
-            check(self._lib.axkv_pages_compact(self._ref, n.data_ptr(), ws.data_ptr(), ws.numel(),
-                                               self._stream()))
+        n = torch.empty(1, dtype=torch.int32, device=self._device)
+        ws = self._workspace(0)
+        self._call(self._lib.axkv_pages_compact, n.data_ptr(), ws.data_ptr(), ws.numel())
         return n
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Page src[i] to page dst[i] in every pool (no destination twice, none a source)."""
-        a, b = self._ints("src and dst", src, dst)
-        with _on(self.block_table.device):
-            check(self._lib.axkv_pages_copy(self._ref, a, b, src.shape[0], self._stream()))
+        n, at = self._list(src, dst)
+        self._call(self._lib.axkv_pages_copy, *at, n)

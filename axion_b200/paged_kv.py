@@ -9,7 +9,6 @@ sequence s owns pages s * max_blocks onwards (identity block table).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import torch
@@ -130,13 +129,50 @@ class PagedKVCache:
         return out
 
 
-def _on(device: torch.device):
-    """The device of the cache as the current one, for the length of a call."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index \
-        else torch.cuda.device(device)
+class _DeviceCalls:
+    """Argument checks and the current stream of the objects below.  A call takes
+    a few microseconds on the device, so these stay off the slower torch paths."""
+
+    _what = ""
+
+    def _set_device(self, t: torch.Tensor) -> None:
+        self._dev = t.get_device()
+        self._device = t.device
+
+    def _ints(self, t: torch.Tensor | None, n: int, what: str) -> int | None:
+        """The address of n contiguous int32 on the object's device (None stays)."""
+        if t is None:
+            return None
+        if t.dtype is not torch.int32 or t.get_device() != self._dev or t.dim() != 1 \
+                or t.shape[0] != n or not t.is_contiguous():
+            raise RuntimeError(f"{self._what}: {what} must be contiguous int32 [{n}] on the "
+                               "device of the object's tensors")
+        return t.data_ptr()
+
+    def _call(self, fn, *args) -> None:
+        """fn(self._ref, *args, stream) on the object's device and its current stream."""
+        stream = torch._C._cuda_getCurrentRawStream(self._dev)
+        if torch._C._cuda_getDevice() == self._dev:
+            rc = fn(self._ref, *args, stream)
+        else:
+            with torch.cuda.device(self._device):
+                rc = fn(self._ref, *args, stream)
+        if rc:
+            check(rc)
+
+    def _scratch(self, need: int) -> torch.Tensor:
+        """A workspace of `need` bytes for one call: kept per stream, on which
+        calls follow one another; a captured graph's is its own."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(need, dtype=torch.uint8, device=self._device)
+        key = torch._C._cuda_getCurrentRawStream(self._dev)
+        ws = self._ws.get(key)
+        if ws is None or ws.numel() < need:
+            ws = self._ws[key] = torch.empty(need, dtype=torch.uint8, device=self._device)
+        return ws
 
 
-class PagedKVCache4:
+class PagedKVCache4(_DeviceCalls):
     """The paged cache in 4 bits (include/axkv.h, axkv4_cache): K and V as 4-bit
     codes with a step and a zero point per token and 32 dims, 0.5625 byte per
     value, under the method names of :class:`PagedKVCache`.
@@ -149,12 +185,13 @@ class PagedKVCache4:
     manages; sequences and positions are then named by the caller
     (``append_rows``, ``decode_attention``, ``chunk_attention``).
 
-    Calls go to the current stream of the cache's device.  Workspaces come from
-    torch's allocator, a call's own: calls of one cache on several streams and
-    captured graphs may run at once.
+    Calls go to the current stream of the cache's device.  Each stream and each
+    captured graph has a workspace of its own, so calls of one cache on several
+    streams and replayed graphs may run at once.
     """
 
     page_size = 16
+    _what = "PagedKVCache4"
 
     def __init__(self, n_kv_heads: int, head_dim: int, max_seqs: int = 1, max_tokens: int = 4096,
                  device=None, *, pages: torch.Tensor | None = None,
@@ -192,34 +229,27 @@ class PagedKVCache4:
                                     self.max_blocks, pages.shape[0], n_kv_heads, head_dim,
                                     self.page_size)
         self._ref = C.byref(self.c)
+        self._set_device(pages)
+        self._ws: dict[int, torch.Tensor] = {}
         self._need: dict[tuple, int] = {}
         self._lib = _lib.load()
 
     # -- arguments ---------------------------------------------------------------
-    def _ints(self, t: torch.Tensor | None, n: int, what: str) -> int | None:
-        if t is None:
-            return None
-        if t.dtype != torch.int32 or t.device != self.pages.device or t.dim() != 1 \
-                or t.shape[0] != n or not t.is_contiguous():
-            raise RuntimeError(f"PagedKVCache4: {what} must be contiguous int32 [{n}] on the "
-                               "cache's device")
-        return t.data_ptr()
-
     def _rows(self, t: torch.Tensor, width: int, what: str) -> torch.Tensor:
         """fp32 rows [n, width], 16-byte aligned, with a row pitch the kernels take."""
-        if t.dim() != 2 or t.shape[1] != width or t.device != self.pages.device:
+        if t.dim() != 2 or t.shape[1] != width or t.get_device() != self._dev:
             raise RuntimeError(f"PagedKVCache4: {what} must be [rows, {width}] on the cache's device")
-        if t.dtype != torch.float32:
+        if t.dtype is not torch.float32:
             t = t.float()
-        if t.shape[0] and (t.stride(1) != 1 or t.stride(0) % 4 or t.stride(0) < width
-                           or t.data_ptr() % 16):
+        pitch, step = t.stride()
+        if t.shape[0] and (step != 1 or pitch % 4 or pitch < width or t.data_ptr() % 16):
             t = t.clone(memory_format=torch.contiguous_format)
         return t
 
     def _out(self, out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
         if out is None:
-            return torch.empty(q.shape, dtype=torch.float32, device=q.device)
-        if out.shape != q.shape or out.dtype != torch.float32 or out.device != q.device \
+            return torch.empty(q.shape, dtype=torch.float32, device=self._device)
+        if out.shape != q.shape or out.dtype != torch.float32 or out.get_device() != self._dev \
                 or not out.is_contiguous() or out.data_ptr() % 16:
             raise RuntimeError("PagedKVCache4: out must be contiguous fp32 like q, 16-byte aligned")
         return out
@@ -228,14 +258,13 @@ class PagedKVCache4:
         key = (fn.__name__, *sizes)
         need = self._need.get(key)
         if need is None:
-            need = self._need[key] = fn(self._ref, *sizes)
-        if need < 0:
-            raise RuntimeError(_lib.load().axq8_last_error().decode(errors="replace")
-                               or "PagedKVCache4: unsupported attention shape")
-        return torch.empty(need, dtype=torch.uint8, device=self.pages.device)
-
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.pages.device).cuda_stream
+            with torch.cuda.device(self._device):
+                need = fn(self._ref, *sizes)
+            if need < 0:
+                raise RuntimeError(self._lib.axq8_last_error().decode(errors="replace")
+                                   or "PagedKVCache4: unsupported attention shape")
+            self._need[key] = need
+        return self._scratch(need)
 
     # -- rows of a caller's sequences ----------------------------------------------
     def append_rows(self, K: torch.Tensor, V: torch.Tensor, row_seq: torch.Tensor,
@@ -248,21 +277,18 @@ class PagedKVCache4:
             raise RuntimeError("PagedKVCache4: K and V must be [rows, hidden]")
         if n and K.stride(0) != V.stride(0):
             K, V = K.contiguous(), V.contiguous()
-        seq, pos = self._ints(row_seq, n, "row_seq"), self._ints(row_pos, n, "row_pos")
-        with _on(self.pages.device):
-            check(self._lib.axkv4_append(self._ref, K.data_ptr(), V.data_ptr(),
-                                         K.stride(0) if n else self.hidden_size, n, seq, pos,
-                                         self._stream()))
+        self._call(self._lib.axkv4_append, K.data_ptr(), V.data_ptr(),
+                   K.stride(0) if n else self.hidden_size, n, self._ints(row_seq, n, "row_seq"),
+                   self._ints(row_pos, n, "row_pos"))
 
     def read_rows(self, row_seq: torch.Tensor, row_pos: torch.Tensor):
         """The values held at those positions: (K, V) fp32 [n, hidden]."""
         n = row_seq.shape[0]
-        seq, pos = self._ints(row_seq, n, "row_seq"), self._ints(row_pos, n, "row_pos")
-        kv = torch.empty(2, n, self.hidden_size, dtype=torch.float32, device=self.pages.device)
-        with _on(self.pages.device):
-            check(self._lib.axkv4_read(self._ref, kv[0].data_ptr(), kv[1].data_ptr(),
-                                       self.hidden_size, n, seq, pos, self._stream()))
-        return kv[0], kv[1]
+        kv = torch.empty((2, n, self.hidden_size), dtype=torch.float32, device=self._device)
+        k = kv.data_ptr()
+        self._call(self._lib.axkv4_read, k, k + n * self.hidden_size * 4, self.hidden_size, n,
+                   self._ints(row_seq, n, "row_seq"), self._ints(row_pos, n, "row_pos"))
+        return kv.unbind()
 
     def decode_attention(self, q: torch.Tensor, n_heads: int, q_pos: torch.Tensor,
                          q_seq: torch.Tensor | None = None, out: torch.Tensor | None = None):
@@ -273,13 +299,10 @@ class PagedKVCache4:
         n = q.shape[0]
         out = self._out(out, q)
         pos, seq = self._ints(q_pos, n, "q_pos"), self._ints(q_seq, n, "q_seq")
-        if n == 0:
-            return out
-        with _on(self.pages.device):
+        if n:
             ws = self._workspace(self._lib.axkv4_decode_attn_workspace, n, n_heads)
-            check(self._lib.axkv4_decode_attn(self._ref, q.data_ptr(), q.stride(0), n, n_heads, seq,
-                                              pos, out.data_ptr(), ws.data_ptr(), ws.numel(),
-                                              self._stream()))
+            self._call(self._lib.axkv4_decode_attn, q.data_ptr(), q.stride(0), n, n_heads, seq, pos,
+                       out.data_ptr(), ws.data_ptr(), ws.numel())
         return out
 
     def chunk_attention(self, q: torch.Tensor, n_heads: int, q_start: torch.Tensor,
@@ -294,13 +317,10 @@ class PagedKVCache4:
         out = self._out(out, q)
         start = self._ints(q_start, chunks + 1, "q_start")
         pos, seq = self._ints(q_pos, chunks, "q_pos"), self._ints(q_seq, chunks, "q_seq")
-        if n == 0 or chunks == 0 or max_rows == 0:
-            return out
-        with _on(self.pages.device):
+        if n and chunks and max_rows:
             ws = self._workspace(self._lib.axkv4_chunk_attn_workspace, chunks, max_rows, n_heads)
-            check(self._lib.axkv4_chunk_attn(self._ref, q.data_ptr(), q.stride(0), n, chunks,
-                                             max_rows, n_heads, seq, start, pos, out.data_ptr(),
-                                             ws.data_ptr(), ws.numel(), self._stream()))
+            self._call(self._lib.axkv4_chunk_attn, q.data_ptr(), q.stride(0), n, chunks, max_rows,
+                       n_heads, seq, start, pos, out.data_ptr(), ws.data_ptr(), ws.numel())
         return out
 
     # -- the reference's names, sequences filled from their start -------------------
