@@ -30,65 +30,86 @@ __device__ __forceinline__ uint8_t* kv4_at(const Kv4Pages& c, int s, int p, int 
     return c.pages + ((int64_t)page * c.n_kv + h) * Kv4<HD>::BYTES;
 }
 
-// One warp per (row, KV head); lane l holds dim 32 b + l of every block b.
+// Append and read move 4 dims per lane: HD / 4 lanes to a (row, KV head), 8 lanes
+// to a block.  Lane i of a head (dims 4 i ..) has half a K word, and one nibble of
+// 4 bytes of V, whose other nibble is lane i ^ 2's.
+template <int HD>
+struct Kv4Lane {
+    using F = Kv4<HD>;
+    int b, k_at, v_at;   // block, byte offsets of the 4 K codes and of the first V byte in slot 0
+    bool high;           // V codes are the high nibbles
+    __device__ __forceinline__ explicit Kv4Lane(int i) {
+        b = i / 8;
+        k_at = F::k_byte(0, b, 2 * (i % 8));
+        v_at = F::v_byte(0, i / 4, 4 * (i & 1));
+        high = i & 2;
+    }
+    static constexpr int V_STEP = 16 * F::TPG;   // bytes from dim g to g + 1
+    __device__ __forceinline__ int k(int slot) const { return k_at + slot * (HD / 2); }
+    __device__ __forceinline__ int v(int slot) const { return v_at + F::v_byte(slot, 0, 0) - F::V; }
+};
+
+// Bound: HBM (4 + 0.5625 bytes a value); one read of the rows, all in registers.
 template <int HD>
 __global__ void __launch_bounds__(256)
     kv4_append_kernel(Kv4Pages c, const float* __restrict__ k_rows, const float* __restrict__ v_rows,
                       int64_t ld, int n_rows, const int* __restrict__ row_seq,
                       const int* __restrict__ row_pos, int* __restrict__ status) {
     using F = Kv4<HD>;
-    const int64_t gw = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (gw >= (int64_t)n_rows * c.n_kv) return;
-    const int r = (int)(gw / c.n_kv), h = (int)(gw % c.n_kv);
-    const int p = row_pos[r];
-    uint8_t* base = kv4_at<HD>(c, row_seq[r], p, h);
-    if (!base) {
-        if (lane == 0) record_status(status, AXQ8_ERR_INVALID);
-        return;
-    }
-    const int slot = p % kKv4Tokens;
+    constexpr int LPR = HD / 4;
+    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LPR;
+    const int i = threadIdx.x % LPR;
+    const bool in = unit < (int64_t)n_rows * c.n_kv;
+    const int r = in ? (int)(unit / c.n_kv) : 0, h = in ? (int)(unit % c.n_kv) : 0;
+    const int64_t src = (int64_t)r * ld + (int64_t)h * HD + 4 * i;
+    const float4 kx = __ldg(reinterpret_cast<const float4*>(k_rows + src));
+    const float4 vx = __ldg(reinterpret_cast<const float4*>(v_rows + src));
+    const int p = row_pos[r], slot = p & (kKv4Tokens - 1);
+    uint8_t* base = in ? kv4_at<HD>(c, row_seq[r], p, h) : nullptr;
+    if (in && !base && i == 0) record_status(status, AXQ8_ERR_INVALID);
+    const Kv4Lane<HD> at(i);
     bool bad = false;
 #pragma unroll
     for (int kv = 0; kv < 2; kv++) {
-        const float* src = (kv ? v_rows : k_rows) + (int64_t)r * ld + (int64_t)h * HD;
+        float x[4] = {kv ? vx.x : kx.x, kv ? vx.y : kx.y, kv ? vx.z : kx.z, kv ? vx.w : kx.w};
+        float lo = 0.0f, hi = 0.0f;
 #pragma unroll
-        for (int b = 0; b < F::NB; b++) {
-            const float x = kv4_clean(src[32 * b + lane], bad);
-            float lo = fminf(x, 0.0f), hi = fmaxf(x, 0.0f);
+        for (int e = 0; e < 4; e++) {
+            x[e] = kv4_clean(x[e], bad);
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+        }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            }
-            const int code = kv4_step_code(hi - lo);
-            const float d = code ? kv4_step(code) : 1.0f;   // all zero: any step does
-            const float inv = 1.0f / d;
-            const float z = -kv4_round(lo, d, inv);
-            const uint32_t q = (uint32_t)fminf(kv4_round(x, d, inv) + z, 15.0f);
-            if (lane == 0)
-                *reinterpret_cast<uint16_t*>(base + (kv ? F::VS : F::KS) + F::scale(slot, b)) =
-                    (uint16_t)((code << 4) | (int)z);
-            if (kv == 0) {
-                const uint32_t pair = q | (__shfl_down_sync(0xffffffffu, q, 1) << 4);
-                if ((lane & 1) == 0) base[F::k_byte(slot, b, lane >> 1)] = (uint8_t)pair;
-            } else {
-                const uint32_t pair = q | (__shfl_down_sync(0xffffffffu, q, 8) << 4);
-                if ((lane & 8) == 0) base[F::v_byte(slot, 2 * b + (lane >> 4), lane & 7)] = (uint8_t)pair;
+        for (int o = 4; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const int code = kv4_step_code(hi - lo);
+        const float d = code ? kv4_step(code) : 1.0f;   // all zero: any step does
+        const float inv = 1.0f / d;
+        const float z = -kv4_round(lo, d, inv);
+        uint32_t q = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) q |= (uint32_t)fminf(kv4_round(x[e], d, inv) + z, 15.0f) << (4 * e);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, q, 2);
+        if (!base) continue;
+        if (i % 8 == 0)
+            *reinterpret_cast<uint16_t*>(base + (kv ? F::VS : F::KS) + F::scale(slot, at.b)) =
+                (uint16_t)((code << 4) | (int)z);
+        if (kv == 0) {
+            *reinterpret_cast<uint16_t*>(base + at.k(slot)) = (uint16_t)q;
+        } else {
+            // the pair of lanes writes two of the four bytes each
+            const uint32_t l = at.high ? other : q, u = at.high ? q : other;
+            uint8_t* to = base + at.v(slot);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int g = e + (at.high ? 2 : 0);
+                to[g * at.V_STEP] = (uint8_t)(((l >> (4 * g)) & 15) | ((u >> (4 * g)) & 15) << 4);
             }
         }
     }
-    if (__any_sync(0xffffffffu, bad) && lane == 0) record_status(status, AXQ8_ERR_INVALID);
-}
-
-// Dim 32 b + lane of token r of a (page, KV head).
-template <int HD>
-__device__ __forceinline__ float kv4_value(const uint8_t* base, bool v, int r, int b, int lane) {
-    using F = Kv4<HD>;
-    const uint32_t w = *reinterpret_cast<const uint16_t*>(base + (v ? F::VS : F::KS) + F::scale(r, b));
-    const int q = v ? (base[F::v_byte(r, 2 * b + (lane >> 4), lane & 7)] >> ((lane & 8) >> 1)) & 15
-                    : (base[F::k_byte(r, b, lane >> 1)] >> (4 * (lane & 1))) & 15;
-    return kv4_step(w >> 4) * (float)(q - (int)(w & 15));
+    if (in && base && bad) record_status(status, AXQ8_ERR_INVALID);
 }
 
 template <int HD>
@@ -96,19 +117,32 @@ __global__ void __launch_bounds__(256)
     kv4_read_kernel(Kv4Pages c, float* __restrict__ k_rows, float* __restrict__ v_rows, int64_t ld,
                     int n_rows, const int* __restrict__ row_seq, const int* __restrict__ row_pos,
                     int* __restrict__ status) {
-    const int64_t gw = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (gw >= (int64_t)n_rows * c.n_kv) return;
-    const int r = (int)(gw / c.n_kv), h = (int)(gw % c.n_kv);
-    const int p = row_pos[r];
+    using F = Kv4<HD>;
+    constexpr int LPR = HD / 4;
+    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LPR;
+    const int i = threadIdx.x % LPR;
+    if (unit >= (int64_t)n_rows * c.n_kv) return;
+    const int r = (int)(unit / c.n_kv), h = (int)(unit % c.n_kv);
+    const int p = row_pos[r], slot = p & (kKv4Tokens - 1);
     const uint8_t* base = kv4_at<HD>(c, row_seq[r], p, h);
-    if (!base && lane == 0) record_status(status, AXQ8_ERR_INVALID);
+    float k[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (base) {
+        const Kv4Lane<HD> at(i);
+        const int ks = *reinterpret_cast<const uint16_t*>(base + F::KS + F::scale(slot, at.b));
+        const int vs = *reinterpret_cast<const uint16_t*>(base + F::VS + F::scale(slot, at.b));
+        const int kq = *reinterpret_cast<const uint16_t*>(base + at.k(slot));
 #pragma unroll
-    for (int b = 0; b < Kv4<HD>::NB; b++) {
-        const int64_t at = (int64_t)r * ld + (int64_t)h * HD + 32 * b + lane;
-        k_rows[at] = base ? kv4_value<HD>(base, false, p % kKv4Tokens, b, lane) : 0.0f;
-        v_rows[at] = base ? kv4_value<HD>(base, true, p % kKv4Tokens, b, lane) : 0.0f;
+        for (int e = 0; e < 4; e++) {
+            const int vq = base[at.v(slot) + e * at.V_STEP] >> (at.high ? 4 : 0);
+            k[e] = kv4_step(ks >> 4) * (float)(((kq >> (4 * e)) & 15) - (ks & 15));
+            v[e] = kv4_step(vs >> 4) * (float)((vq & 15) - (vs & 15));
+        }
+    } else if (i == 0) {
+        record_status(status, AXQ8_ERR_INVALID);
     }
+    const int64_t to = (int64_t)r * ld + (int64_t)h * HD + 4 * i;
+    *reinterpret_cast<float4*>(k_rows + to) = make_float4(k[0], k[1], k[2], k[3]);
+    *reinterpret_cast<float4*>(v_rows + to) = make_float4(v[0], v[1], v[2], v[3]);
 }
 
 int check_cache4(const axkv4_cache_t* c, const char* what) {
@@ -163,16 +197,16 @@ int check_attn(const axkv4_cache_t* c, const char* what, int32_t n_heads) {
 template <int HD>
 cudaError_t launch_append(const axkv4_cache_t* c, const float* k, const float* v, int64_t ld, int n_rows,
                           const int* seq, const int* pos, int* status, cudaStream_t s) {
-    const int64_t warps = (int64_t)n_rows * c->n_kv_heads;
-    return launch_k(kv4_append_kernel<HD>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, false,
+    const int64_t threads = (int64_t)n_rows * c->n_kv_heads * (HD / 4);
+    return launch_k(kv4_append_kernel<HD>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, false,
                     pages_of(c), k, v, ld, n_rows, seq, pos, status);
 }
 
 template <int HD>
 cudaError_t launch_read(const axkv4_cache_t* c, float* k, float* v, int64_t ld, int n_rows,
                         const int* seq, const int* pos, int* status, cudaStream_t s) {
-    const int64_t warps = (int64_t)n_rows * c->n_kv_heads;
-    return launch_k(kv4_read_kernel<HD>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, false,
+    const int64_t threads = (int64_t)n_rows * c->n_kv_heads * (HD / 4);
+    return launch_k(kv4_read_kernel<HD>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, false,
                     pages_of(c), k, v, ld, n_rows, seq, pos, status);
 }
 

@@ -248,7 +248,7 @@ class PagedKVCache4(_DeviceCalls):
 
     def _out(self, out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
         if out is None:
-            return torch.empty(q.shape, dtype=torch.float32, device=self._device)
+            return q.new_empty(q.shape)
         if out.shape != q.shape or out.dtype != torch.float32 or out.get_device() != self._dev \
                 or not out.is_contiguous() or out.data_ptr() % 16:
             raise RuntimeError("PagedKVCache4: out must be contiguous fp32 like q, 16-byte aligned")
