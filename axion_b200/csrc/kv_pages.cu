@@ -20,7 +20,9 @@ namespace {
 
 constexpr int kPageTokens = 16;
 constexpr int kPlanThreads = 1024;
-constexpr int kPiece = 8192;   // bytes of a page that one CTA copies at a time
+constexpr int kCopyThreads = 256;
+constexpr int kCopyAhead = 4;    // 16-byte loads of a thread on their way
+constexpr int kPiece = kCopyThreads * kCopyAhead * 16;   // bytes of a page that one CTA copies at a time
 
 // Workspace: header, then claim [n_seqs], first [n + 1], src and dst [n_pages]
 // each (compact: + to [n_pages]).
@@ -97,6 +99,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     __shared__ int bad;
     const Plan a = plan_of(ws, p.n_seqs, n, p.n_pages);
     const int tid = threadIdx.x;
+    pdl_launch_dependents();
     for (int i = tid; i < p.n_seqs; i += kPlanThreads) a.claim[i] = 0x7fffffff;
     if (tid == 0) bad = 0;
     __syncthreads();
@@ -135,6 +138,9 @@ __global__ void __launch_bounds__(kPlanThreads)
         }
         int sum;
         const int at = cta_scan(need, sm, &sum);
+        // the page that a fork copies in part; none for a child without one
+        if (FORK && i < n && need && total + at < p.n_pages)
+            a.src[total + at] = __ldcg(p.block_table + (int64_t)parents[i] * p.max_blocks + tokens[i] / kPageTokens);
         if (i < n) a.first[i] = (int)min((int64_t)total + at, (int64_t)p.n_pages + 1);
         total = (int)min((int64_t)total + sum, (int64_t)p.n_pages + 1);
     }
@@ -158,22 +164,53 @@ __global__ void __launch_bounds__(kPlanThreads)
     }
 }
 
-// Piece `at` of page src to page dst of pool `pool`.
-__device__ __forceinline__ void copy_piece(const axkv_pages_t& p, int pool, int src, int dst, int64_t at) {
-    const uint8_t* base = static_cast<const uint8_t*>(p.pools[pool]);
-    const uint4* s = reinterpret_cast<const uint4*>(base + (int64_t)src * p.page_bytes + at);
-    uint4* d = reinterpret_cast<uint4*>(const_cast<uint8_t*>(base) + (int64_t)dst * p.page_bytes + at);
-    const int n = (int)min((int64_t)kPiece, p.page_bytes - at) / 16;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) d[i] = __ldcg(s + i);
+// Pages src[i] to dst[i] in every pool, i < n, over the whole grid in pieces.  Bound:
+// HBM, twice the pages' bytes; the next piece's page numbers are read while a
+// piece is copied.  Pairs outside the pool are left out; reported, if status is.
+__device__ __forceinline__ void copy_pages(const axkv_pages_t& p, const int* src, const int* dst, int n,
+                                           int* status) {
+    if (p.n_pools == 0) return;
+    const int pieces = (int)((p.page_bytes + kPiece - 1) / kPiece);
+    const int64_t items = (int64_t)n * p.n_pools * pieces;
+    int64_t it = blockIdx.x;
+    if (it >= items) return;
+    int i = (int)(it / pieces / p.n_pools), s = __ldcg(src + i), d = __ldcg(dst + i);
+    for (;;) {
+        const int piece = (int)(it % pieces), pool = (int)(it / pieces % p.n_pools);
+        const int64_t next = it + gridDim.x;
+        const int i2 = next < items ? (int)(next / pieces / p.n_pools) : i;
+        const int s2 = __ldcg(src + i2), d2 = __ldcg(dst + i2);
+        if ((unsigned)s < (unsigned)p.n_pages && (unsigned)d < (unsigned)p.n_pages) {
+            const int64_t at = (int64_t)piece * kPiece;
+            uint8_t* base = static_cast<uint8_t*>(p.pools[pool]);
+            const uint4* from = reinterpret_cast<const uint4*>(base + (int64_t)s * p.page_bytes + at);
+            uint4* to = reinterpret_cast<uint4*>(base + (int64_t)d * p.page_bytes + at);
+            const int words = (int)min((int64_t)kPiece, p.page_bytes - at) / 16;
+            uint4 v[kCopyAhead];
+#pragma unroll
+            for (int k = 0; k < kCopyAhead; k++)
+                if (threadIdx.x + k * kCopyThreads < words) v[k] = __ldcg(from + threadIdx.x + k * kCopyThreads);
+#pragma unroll
+            for (int k = 0; k < kCopyAhead; k++)
+                if (threadIdx.x + k * kCopyThreads < words) to[threadIdx.x + k * kCopyThreads] = v[k];
+        } else if (status && threadIdx.x == 0) {
+            record_status(status, AXQ8_ERR_INVALID);
+        }
+        if (next >= items) return;
+        it = next;
+        s = s2;
+        d = d2;
+    }
 }
 
 // Reserve: the new pages into the rows.  Fork: the children's rows, the counts
 // of the shared pages, and the copies of the partly filled ones.
 template <bool FORK>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kCopyThreads)
     pages_apply_kernel(axkv_pages_t p, const int* __restrict__ parents, const int* __restrict__ seqs,
                        const int* __restrict__ tokens, int n, void* ws) {
     const Plan a = plan_of(ws, p.n_seqs, n, p.n_pages);
+    pdl_wait();
     if (!__ldcg(a.header + 1)) return;
     const int step = gridDim.x * (blockDim.x >> 5);
     const int lane = threadIdx.x & 31;
@@ -202,21 +239,10 @@ __global__ void __launch_bounds__(256)
             }
         }
     }
-    if (!FORK) return;
-    const int pieces = (int)((p.page_bytes + kPiece - 1) / kPiece);
-    const int64_t items = (int64_t)n * p.n_pools * pieces;
-    for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        const int piece = (int)(it % pieces), pool = (int)(it / pieces % p.n_pools);
-        const int i = (int)(it / pieces / p.n_pools);
-        const int f0 = __ldcg(a.first + i);
-        if (__ldcg(a.first + i + 1) == f0) continue;
-        const int src = __ldcg(p.block_table + (int64_t)parents[i] * p.max_blocks + tokens[i] / kPageTokens);
-        if (src >= 0 && src < p.n_pages)
-            copy_piece(p, pool, src, __ldcg(a.dst + f0), (int64_t)piece * kPiece);
-    }
+    if (FORK) copy_pages(p, a.src, a.dst, __ldcg(a.header), nullptr);
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kCopyThreads)
     pages_free_kernel(axkv_pages_t p, const int* __restrict__ seqs, int n, int* __restrict__ status) {
     const int lane = threadIdx.x & 31;
     const int step = gridDim.x * (blockDim.x >> 5);
@@ -241,6 +267,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     __shared__ int sm[32];
     const Plan a = plan_of(ws, p.n_seqs, 0, p.n_pages);
     const int tid = threadIdx.x;
+    pdl_launch_dependents();
     int mine = 0, live;
     for (int g = tid; g < p.n_pages; g += kPlanThreads) mine += __ldcg(p.ref_count + g) > 0;
     cta_scan(mine, sm, &live);
@@ -271,8 +298,9 @@ __global__ void __launch_bounds__(kPlanThreads)
     }
 }
 
-__global__ void __launch_bounds__(256) pages_move_kernel(axkv_pages_t p, void* ws) {
+__global__ void __launch_bounds__(kCopyThreads) pages_move_kernel(axkv_pages_t p, void* ws) {
     const Plan a = plan_of(ws, p.n_seqs, 0, p.n_pages);
+    pdl_wait();
     const int ns = __ldcg(a.header), live = __ldcg(a.header + 2);
     const int64_t entries = (int64_t)p.n_seqs * p.max_blocks;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < entries;
@@ -280,30 +308,13 @@ __global__ void __launch_bounds__(256) pages_move_kernel(axkv_pages_t p, void* w
         const int page = p.block_table[i];
         if (page >= live && page < p.n_pages) p.block_table[i] = __ldcg(a.to + page);
     }
-    const int pieces = (int)((p.page_bytes + kPiece - 1) / kPiece);
-    const int64_t items = (int64_t)ns * p.n_pools * pieces;
-    for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        const int piece = (int)(it % pieces), pool = (int)(it / pieces % p.n_pools);
-        const int k = (int)(it / pieces / p.n_pools);
-        copy_piece(p, pool, __ldcg(a.src + k), __ldcg(a.dst + k), (int64_t)piece * kPiece);
-    }
+    copy_pages(p, a.src, a.dst, ns, nullptr);
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kCopyThreads)
     pages_copy_kernel(axkv_pages_t p, const int* __restrict__ src, const int* __restrict__ dst, int n,
                       int* __restrict__ status) {
-    const int pieces = (int)((p.page_bytes + kPiece - 1) / kPiece);
-    const int64_t items = (int64_t)n * p.n_pools * pieces;
-    for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        const int piece = (int)(it % pieces), pool = (int)(it / pieces % p.n_pools);
-        const int i = (int)(it / pieces / p.n_pools);
-        const int s = src[i], d = dst[i];
-        if (s < 0 || s >= p.n_pages || d < 0 || d >= p.n_pages) {
-            if (threadIdx.x == 0) record_status(status, AXQ8_ERR_INVALID);
-            continue;
-        }
-        copy_piece(p, pool, s, d, (int64_t)piece * kPiece);
-    }
+    copy_pages(p, src, dst, n, status);
 }
 
 int check_pages(const axkv_pages_t* p, const char* what) {
@@ -353,7 +364,7 @@ int allocate(const axkv_pages_t* p, const char* what, const int32_t* parents, co
                   "axkv_pages plan launch");
     const int64_t items = FORK ? (int64_t)n * p->n_pools * pieces_of(p) : 0;
     AXQ8_CUDA_TRY(launch_k(pages_apply_kernel<FORK>, dim3(copy_ctas(ds, std::max<int64_t>(items, (n + 7) / 8))),
-                           dim3(256), 0, s, false, *p, parents, seqs, tokens, (int)n, ws),
+                           dim3(kCopyThreads), 0, s, true, *p, parents, seqs, tokens, (int)n, ws),
                   "axkv_pages apply launch");
     return AXQ8_OK;
 }
@@ -388,7 +399,7 @@ int axkv_pages_free(const axkv_pages_t* p, const int32_t* seqs, int32_t n, void*
     if (!seqs) return fail(AXQ8_ERR_INVALID, "axkv_pages_free: null pointer");
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
-    AXQ8_CUDA_TRY(launch_k(pages_free_kernel, dim3(copy_ctas(ds, (n + 7) / 8)), dim3(256), 0,
+    AXQ8_CUDA_TRY(launch_k(pages_free_kernel, dim3(copy_ctas(ds, (n + 7) / 8)), dim3(kCopyThreads), 0,
                            static_cast<cudaStream_t>(stream), false, *p, seqs, (int)n, ds->status),
                   "axkv_pages_free launch");
     return AXQ8_OK;
@@ -407,7 +418,7 @@ int axkv_pages_compact(const axkv_pages_t* p, int32_t* n_live, void* workspace,
                   "axkv_pages_compact plan launch");
     const int64_t items = std::max<int64_t>((int64_t)p->n_pages * p->n_pools * pieces_of(p) / 2,
                                             ((int64_t)p->n_seqs * p->max_blocks + 255) / 256);
-    AXQ8_CUDA_TRY(launch_k(pages_move_kernel, dim3(copy_ctas(ds, items)), dim3(256), 0, s, false, *p,
+    AXQ8_CUDA_TRY(launch_k(pages_move_kernel, dim3(copy_ctas(ds, items)), dim3(kCopyThreads), 0, s, true, *p,
                            workspace),
                   "axkv_pages_compact launch");
     return AXQ8_OK;
@@ -423,7 +434,7 @@ int axkv_pages_copy(const axkv_pages_t* p, const int32_t* src, const int32_t* ds
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
     AXQ8_CUDA_TRY(launch_k(pages_copy_kernel, dim3(copy_ctas(ds, (int64_t)n * p->n_pools * pieces_of(p))),
-                           dim3(256), 0, static_cast<cudaStream_t>(stream), false, *p, src, dst, (int)n,
+                           dim3(kCopyThreads), 0, static_cast<cudaStream_t>(stream), false, *p, src, dst, (int)n,
                            ds->status),
                   "axkv_pages_copy launch");
     return AXQ8_OK;
