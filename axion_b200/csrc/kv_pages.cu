@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kPageTokens = 16;
 constexpr int kPlanThreads = 1024;
+constexpr int kScanPages = 8;     // consecutive pages of a thread in a scan over the counts
 constexpr int kCopyThreads = 256;
 constexpr int kCopyAhead = 4;    // 16-byte loads of a thread on their way
 constexpr int kPiece = kCopyThreads * kCopyAhead * 16;   // bytes of a page that one CTA copies at a time
@@ -147,12 +148,15 @@ __global__ void __launch_bounds__(kPlanThreads)
     if (tid == 0) a.first[n] = total;
     // the lowest `total` free pages
     int found = 0;
-    for (int g0 = 0; g0 < p.n_pages && found < total; g0 += kPlanThreads) {
-        const int g = g0 + tid;
-        const int free = g < p.n_pages && __ldcg(p.ref_count + g) == 0;
+    for (int g0 = 0; g0 < p.n_pages && found < total; g0 += kPlanThreads * kScanPages) {
+        const int g = g0 + tid * kScanPages;
+        unsigned free = 0;
+#pragma unroll
+        for (int k = 0; k < kScanPages; k++)
+            if (g + k < p.n_pages && __ldcg(p.ref_count + g + k) == 0) free |= 1u << k;
         int sum;
-        const int at = found + cta_scan(free, sm, &sum);
-        if (free && at < total) a.dst[at] = g;
+        int at = found + cta_scan(__popc(free), sm, &sum);
+        for (; free && at < total; free &= free - 1) a.dst[at++] = g + __ffs(free) - 1;
         found += sum;
     }
     __syncthreads();
@@ -269,18 +273,28 @@ __global__ void __launch_bounds__(kPlanThreads)
     const int tid = threadIdx.x;
     pdl_launch_dependents();
     int mine = 0, live;
-    for (int g = tid; g < p.n_pages; g += kPlanThreads) mine += __ldcg(p.ref_count + g) > 0;
+#pragma unroll 8
+    for (int g = tid; g < p.n_pages; g += kPlanThreads) {
+        mine += __ldcg(p.ref_count + g) > 0;
+        a.to[g] = g;
+    }
     cta_scan(mine, sm, &live);
     int ns = 0, nd = 0;
-    for (int g0 = 0; g0 < p.n_pages; g0 += kPlanThreads) {
-        const int g = g0 + tid;
-        const bool used = g < p.n_pages && __ldcg(p.ref_count + g) > 0;
-        const int is_src = used && g >= live, is_dst = g < live && !used;
+    for (int g0 = 0; g0 < p.n_pages; g0 += kPlanThreads * kScanPages) {
+        const int g = g0 + tid * kScanPages;
+        unsigned src = 0, dst = 0;
+#pragma unroll
+        for (int k = 0; k < kScanPages; k++) {
+            if (g + k >= p.n_pages) continue;
+            const bool used = __ldcg(p.ref_count + g + k) > 0;
+            if (used && g + k >= live) src |= 1u << k;
+            if (!used && g + k < live) dst |= 1u << k;
+        }
         int sum;
-        const int at = cta_scan(is_src | (is_dst << 16), sm, &sum);
-        if (is_src) a.src[ns + (at & 0xffff)] = g;
-        if (is_dst) a.dst[nd + (at >> 16)] = g;
-        if (g < p.n_pages) a.to[g] = g;
+        const int at = cta_scan(__popc(src) | (__popc(dst) << 16), sm, &sum);   // at most 8192 of each
+        int i = ns + (at & 0xffff), j = nd + (at >> 16);
+        for (; src; src &= src - 1) a.src[i++] = g + __ffs(src) - 1;
+        for (; dst; dst &= dst - 1) a.dst[j++] = g + __ffs(dst) - 1;
         ns += sum & 0xffff;
         nd += sum >> 16;
     }
