@@ -227,7 +227,8 @@ NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int entries, int
     // every tile starts a run where that leaves half of the runs; with the most
     // tiles a call can have (it may have fewer), this many runs are never exceeded
     p.aligned = 2 * tiles <= slots ? (int)tiles : 0;
-    const int64_t runs = (tiles * c->max_blocks + kNarrowMinPages - 1) / kNarrowMinPages + p.aligned;
+    const int64_t runs = p.aligned ? (tiles * c->max_blocks + kNarrowMinPages - 1) / kNarrowMinPages + p.aligned
+                                   : (tiles * (c->max_blocks + kNarrowTileCost) + kNarrowMinUnits - 1) / kNarrowMinUnits;
     p.ctas = (int)std::min<int64_t>(slots, runs);
     p.units = tiles * (c->max_blocks + kNarrowTileCost) * 2;
     p.records = ((int64_t)p.ctas * sizeof(NarrowPart) + 15) / 16 * 16;
@@ -317,9 +318,15 @@ cudaError_t launch_wide(DeviceState* ds, const axkv4_cache_t* c, const float* q,
                     dim3(kWideThreads), smem, s, false, a);
 }
 
-// Columns (rows x heads of a KV head) of a chunk from which the tensor-core
-// tiles of 128 rows take it.
-constexpr int kWideCols = 33;
+// Whether the tensor-core tiles of 256 rows (kv4_wide.cuh) take a chunk call, or the
+// column tiles of 16 (kv4_narrow.cuh), which share a long context among all SMs.
+// Measured per page of context: a CTA of the first takes 0.58 us, whatever its
+// rows, one to an SM; a tile of the second 0.27 us of an SM.
+bool wide_takes(DeviceState* ds, const axkv4_cache_t* c, int chunks, int rows, int G) {
+    const int64_t cols = (int64_t)rows * G, lists = (int64_t)chunks * c->n_kv_heads;
+    const int64_t waves = (lists * ((cols + 255) / 256) + ds->sm_count - 1) / ds->sm_count;
+    return 58 * waves * ds->sm_count < 27 * lists * ((cols + 15) / 16);
+}
 
 }  // namespace
 
@@ -393,9 +400,9 @@ int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32
 int64_t axkv4_chunk_attn_workspace(const axkv4_cache_t* c, int32_t n_chunks, int32_t max_rows,
                                    int32_t n_heads) {
     if (check_attn(c, "axkv4_chunk_attn_workspace", n_heads) || n_chunks <= 0 || max_rows <= 0) return -1;
-    if ((int64_t)max_rows * (n_heads / c->n_kv_heads) >= kWideCols) return 16;
     DeviceState* ds = device_state();
     if (!ds) return -1;
+    if (wide_takes(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads)) return 16;
     return narrow_plan(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads).workspace;
 }
 
@@ -420,7 +427,7 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
     if (workspace_bytes <= 0) return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: no workspace");
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
-    if ((int64_t)max_rows * (n_heads / c->n_kv_heads) >= kWideCols) {
+    if (wide_takes(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads)) {
         if (c->n_kv_heads > 65535) return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d KV heads", c->n_kv_heads);
         AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_wide, ds, c, q, ldq, n_rows, n_chunks, max_rows, n_heads,
                                       q_seq, q_start, q_pos, out,

@@ -48,7 +48,8 @@ namespace axq8 {
 
 constexpr int kNarrowWarps = 4;
 constexpr int kNarrowPages = 4;       // page buffers of a warp
-constexpr int kNarrowMinPages = 24;   // pages of a run at least
+constexpr int kNarrowMinPages = 24;   // pages of a run at least, where every tile starts one
+constexpr int kNarrowMinUnits = 14;   // units of a run at least elsewhere
 constexpr int kNarrowMaxParts = 96;   // parts of a tile at most (one CTA joins them)
 constexpr int kJoinThreads = 256;
 constexpr int kNarrowTileCost = 10;   // what a tile costs beside its pages, in pages
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
             if (pass) break;
             // aligned: at most `tiles` more runs than the units fill
             const int ctas = gridDim.x - a.aligned;
-            run = max(max(kNarrowMinPages, (total + ctas - 1) / ctas), (longest + kNarrowMaxParts - 1) / kNarrowMaxParts);
+            run = max(max(a.aligned ? kNarrowMinPages : kNarrowMinUnits, (total + ctas - 1) / ctas), (longest + kNarrowMaxParts - 1) / kNarrowMaxParts);
             if (!a.aligned) break;
         }
         const int p = blockIdx.x * run;
