@@ -57,7 +57,6 @@ class KVPages(_DeviceCalls):
                                    self.max_blocks, n_pages)
         self._ref = C.byref(self.c)
         self._set_device(block_table)
-        self._ws: dict[int, torch.Tensor] = {}
         self._lib = _lib.load()
         self._need = self._lib.axkv_pages_workspace(self._ref, 0)
 
@@ -75,21 +74,16 @@ class KVPages(_DeviceCalls):
         n = ts[0].shape[0] if ts[0].dim() == 1 else -1
         return n, [self._ints(t, n, "requests") for t in ts]
 
-    def _workspace(self, n: int) -> torch.Tensor:
-        return self._scratch(self._need + 4 * n)
-
     def reserve(self, seqs: torch.Tensor, tokens: torch.Tensor) -> None:
         """Pages for tokens[i] tokens of sequence seqs[i] (each named once)."""
         n, at = self._list(seqs, tokens)
-        ws = self._workspace(n)
-        self._call(self._lib.axkv_pages_reserve, *at, n, ws.data_ptr(), ws.numel())
+        self._call_ws(self._need + 4 * n, self._lib.axkv_pages_reserve, *at, n)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor, tokens: torch.Tensor) -> None:
         """Empty sequence children[i] becomes a copy of the first tokens[i]
         tokens of parents[i]: full pages shared, a partly filled one copied."""
         n, at = self._list(parents, children, tokens)
-        ws = self._workspace(n)
-        self._call(self._lib.axkv_pages_fork, *at, n, ws.data_ptr(), ws.numel())
+        self._call_ws(self._need + 4 * n, self._lib.axkv_pages_fork, *at, n)
 
     def free(self, seqs: torch.Tensor) -> None:
         """Sequences give their pages up."""
@@ -99,8 +93,7 @@ class KVPages(_DeviceCalls):
     def compact(self) -> torch.Tensor:
         """Live pages to the front of every pool; their number (int32 [1])."""
         n = torch.empty(1, dtype=torch.int32, device=self._device)
-        ws = self._workspace(0)
-        self._call(self._lib.axkv_pages_compact, n.data_ptr(), ws.data_ptr(), ws.numel())
+        self._call_ws(self._need, self._lib.axkv_pages_compact, n.data_ptr())
         return n
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor) -> None:

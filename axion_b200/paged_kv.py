@@ -10,6 +10,7 @@ sequence s owns pages s * max_blocks onwards (identity block table).
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -138,6 +139,8 @@ class _DeviceCalls:
     def _set_device(self, t: torch.Tensor) -> None:
         self._dev = t.get_device()
         self._device = t.device
+        self._ws: dict[int, torch.Tensor] = {}
+        self._lock = threading.Lock()
 
     def _ints(self, t: torch.Tensor | None, n: int, what: str) -> int | None:
         """The address of n contiguous int32 on the object's device (None stays)."""
@@ -160,16 +163,19 @@ class _DeviceCalls:
         if rc:
             check(rc)
 
-    def _scratch(self, need: int) -> torch.Tensor:
-        """A workspace of `need` bytes for one call: kept per stream, on which
-        calls follow one another; a captured graph's is its own."""
+    def _call_ws(self, need: int, fn, *args) -> None:
+        """_call with a workspace of `need` bytes: kept per stream, on which calls
+        follow one another (the kernels of a call too: threads take turns); a
+        captured graph's is its own."""
         if torch.cuda.is_current_stream_capturing():
-            return torch.empty(need, dtype=torch.uint8, device=self._device)
+            ws = torch.empty(need, dtype=torch.uint8, device=self._device)
+            return self._call(fn, *args, ws.data_ptr(), need)
         key = torch._C._cuda_getCurrentRawStream(self._dev)
-        ws = self._ws.get(key)
-        if ws is None or ws.numel() < need:
-            ws = self._ws[key] = torch.empty(need, dtype=torch.uint8, device=self._device)
-        return ws
+        with self._lock:
+            ws = self._ws.get(key)
+            if ws is None or ws.numel() < need:
+                ws = self._ws[key] = torch.empty(need, dtype=torch.uint8, device=self._device)
+            self._call(fn, *args, ws.data_ptr(), ws.numel())
 
 
 class PagedKVCache4(_DeviceCalls):
@@ -230,7 +236,6 @@ class PagedKVCache4(_DeviceCalls):
                                     self.page_size)
         self._ref = C.byref(self.c)
         self._set_device(pages)
-        self._ws: dict[int, torch.Tensor] = {}
         self._need: dict[tuple, int] = {}
         self._lib = _lib.load()
 
@@ -254,7 +259,8 @@ class PagedKVCache4(_DeviceCalls):
             raise RuntimeError("PagedKVCache4: out must be contiguous fp32 like q, 16-byte aligned")
         return out
 
-    def _workspace(self, fn, *sizes: int) -> torch.Tensor:
+    def _workspace(self, fn, *sizes: int) -> int:
+        """Workspace bytes of a call of these sizes."""
         key = (fn.__name__, *sizes)
         need = self._need.get(key)
         if need is None:
@@ -264,7 +270,7 @@ class PagedKVCache4(_DeviceCalls):
                 raise RuntimeError(self._lib.axq8_last_error().decode(errors="replace")
                                    or "PagedKVCache4: unsupported attention shape")
             self._need[key] = need
-        return self._scratch(need)
+        return need
 
     # -- rows of a caller's sequences ----------------------------------------------
     def append_rows(self, K: torch.Tensor, V: torch.Tensor, row_seq: torch.Tensor,
@@ -300,9 +306,9 @@ class PagedKVCache4(_DeviceCalls):
         out = self._out(out, q)
         pos, seq = self._ints(q_pos, n, "q_pos"), self._ints(q_seq, n, "q_seq")
         if n:
-            ws = self._workspace(self._lib.axkv4_decode_attn_workspace, n, n_heads)
-            self._call(self._lib.axkv4_decode_attn, q.data_ptr(), q.stride(0), n, n_heads, seq, pos,
-                       out.data_ptr(), ws.data_ptr(), ws.numel())
+            need = self._workspace(self._lib.axkv4_decode_attn_workspace, n, n_heads)
+            self._call_ws(need, self._lib.axkv4_decode_attn, q.data_ptr(), q.stride(0), n, n_heads,
+                          seq, pos, out.data_ptr())
         return out
 
     def chunk_attention(self, q: torch.Tensor, n_heads: int, q_start: torch.Tensor,
@@ -318,9 +324,9 @@ class PagedKVCache4(_DeviceCalls):
         start = self._ints(q_start, chunks + 1, "q_start")
         pos, seq = self._ints(q_pos, chunks, "q_pos"), self._ints(q_seq, chunks, "q_seq")
         if n and chunks and max_rows:
-            ws = self._workspace(self._lib.axkv4_chunk_attn_workspace, chunks, max_rows, n_heads)
-            self._call(self._lib.axkv4_chunk_attn, q.data_ptr(), q.stride(0), n, chunks, max_rows,
-                       n_heads, seq, start, pos, out.data_ptr(), ws.data_ptr(), ws.numel())
+            need = self._workspace(self._lib.axkv4_chunk_attn_workspace, chunks, max_rows, n_heads)
+            self._call_ws(need, self._lib.axkv4_chunk_attn, q.data_ptr(), q.stride(0), n, chunks,
+                          max_rows, n_heads, seq, start, pos, out.data_ptr())
         return out
 
     # -- the reference's names, sequences filled from their start -------------------

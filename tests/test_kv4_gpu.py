@@ -352,6 +352,102 @@ def test_chunk_long_past():
         check_rows(case, q[pick], out[pick], 2, [0] * len(pick), [9001 + i for i in pick])
 
 
+# (hd, heads, kv, rows, past): enough rows and KV heads for the tensor-core tiles
+TILES = [(128, 32, 8, (300, 1, 129, 64), (0, 700, 3, 0)), (64, 32, 8, (200, 255, 0, 40), (130, 0, 5, 1)),
+         (32, 16, 16, (400, 33), (0, 250)), (128, 16, 16, (257, 256), (15, 0)), (64, 48, 16, (97, 200), (0, 64)),
+         (64, 56, 8, (130, 131), (17, 0)), (128, 64, 4, (100, 120), (0, 333))]
+
+
+@pytest.mark.parametrize("hd,heads,kv,rows,past", TILES)
+def test_chunk_attention_of_long_chunks(hd, heads, kv, rows, past):
+    """Rows at and beside the tiles' borders, against 64 bits; rows behind the last stay."""
+    rng = np.random.default_rng(hd + heads + rows[0])
+    case = Case(rng, kv, hd, [a + b for a, b in zip(rows, past)], scale=1.5)
+    total = sum(rows)
+    q = (rng.normal(0, 1, (total + 5, heads * hd)) * np.exp2(rng.integers(-3, 3, (total + 5, 1)))).astype(np.float32)
+    start = np.concatenate([[0], np.cumsum(rows)])
+    out = torch.full((total + 5, heads * hd), 7.0, device="cuda")
+    args = (dev(q), heads, ints(start), ints(past), max(rows))
+    case.cache.chunk_attention(*args, out=out)
+    first = out.clone()
+    seqs = np.array([i for i, n in enumerate(rows) for _ in range(n)])
+    ctx = np.array([p + j + 1 for n, p in zip(rows, past) for j in range(n)])
+    border = 128 * kv // heads
+    pick = sorted({int(s + j) for s, n in zip(start, rows) for j in (0, 1, 15, 16, border - 1, border, 2 * border - 1,
+                   2 * border, n // 2, n - 2, n - 1) if 0 <= j < n})
+    check_rows(case, q[pick], out.cpu().numpy()[pick], heads, seqs[pick], ctx[pick])
+    assert bool((out[total:] == 7.0).all()) and status() == 0
+    case.cache.chunk_attention(*args, out=out)
+    assert torch.equal(out, first)                   # bit for bit
+
+
+def test_long_chunks_with_empty_rows_and_bad_pages():
+    """Positions before the start, a page outside the pool, a sequence outside the table."""
+    from axion_b200 import _lib
+    rng = np.random.default_rng(27)
+    case = Case(rng, 8, 64, (300, 300), scale=1.5)
+    case.cache.block_table[1, 9] = 10 ** 6
+    q = rng.normal(0, 1, (900, 32 * 64)).astype(np.float32)
+    out = run_chunks(case, q, 32, (300, 300, 300), (-40, 0, 0), (0, 1, 5)).cpu().numpy()
+    assert status() == _lib.AXQ8_ERR_INVALID
+    assert not out[:40].any() and not out[600:].any()
+    check_rows(case, q[[40, 41, 299]], out[[40, 41, 299]], 32, [0] * 3, [1, 2, 260])
+    check_rows(case, q[[300, 443]], out[[300, 443]], 32, [1] * 2, [1, 144])
+    keep = [p for p in range(300) if p // 16 != 9]
+    case.k[1], case.v[1], case.lens = case.k[1][keep], case.v[1][keep], [300, 284]
+    check_rows(case, q[[450, 599]], out[[450, 599]], 32, [1] * 2, [144, 284])
+
+
+@pytest.mark.parametrize("hd,heads,kv,long", [(128, 16, 4, False), (64, 16, 2, False), (128, 9, 1, False),
+                                              (64, 32, 8, True), (128, 32, 8, True), (32, 16, 16, True)])
+def test_growing_scores_and_values(hd, heads, kv, long):
+    """Scores that grow by 60 and values by 2^12 along the sequence move the softmax reference and
+    the value scale many times; then both fall again."""
+    rng = np.random.default_rng(hd + heads)
+    n = 420
+    case = Case(rng, kv, hd, (n, n))
+    u = rng.normal(0, 1, hd)
+    up = np.concatenate([np.linspace(-30, 30, n // 2), np.linspace(30, -30, n - n // 2)])
+    for s in range(2):
+        case.k[s][:] = (0.3 * case.k[s] + (up * np.sqrt(hd) / (u @ u))[:, None, None] * u).astype(np.float32)
+        case.v[s][:] = case.v[s] * np.exp2(up / 5)[:, None, None].astype(np.float32)
+    case.append(0, None)
+    rows = n if long else 1
+    q = np.tile(u, (2 * rows, heads)).astype(np.float32) * rng.uniform(0.9, 1.1, (2 * rows, 1)).astype(np.float32)
+    past = n - rows
+    if long:
+        out = run_chunks(case, q, heads, (rows, rows), (past, past)).cpu().numpy()
+        pick = [0, 1, 100, 209, 210, 260, n - 1, n, n + 130, 2 * n - 1]
+    else:
+        out = case.cache.decode_attention(dev(q), heads, ints([n - 1, n - 1])).cpu().numpy()
+        pick = [0, 1]
+    check_rows(case, q[pick], out[pick], heads, [r // rows for r in pick], [past + r % rows + 1 for r in pick])
+    assert status() == 0
+
+
+def test_calls_from_two_threads():
+    """Two threads on one cache and one stream: the kernels of their calls do not mix."""
+    import threading
+    rng = np.random.default_rng(28)
+    case = Case(rng, 2, 128, (3000, 2500))
+    qs = [dev(rng.normal(0, 1, (2, 8 * 128)).astype(np.float32)) for _ in range(2)]
+    pos = ints([2999, 2499])
+    want = [case.cache.decode_attention(x, 8, pos) for x in qs]
+    bad = []
+
+    def work(i):
+        for _ in range(200):
+            if not torch.equal(case.cache.decode_attention(qs[i], 8, pos), want[i]):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_masked_slots_do_not_leak():
     """Later tokens of the same page and tile hold the largest values the format has."""
     rng = np.random.default_rng(24)
@@ -365,6 +461,14 @@ def test_masked_slots_do_not_leak():
     check_rows(case, q, out, 8, [0] * n, range(1, n + 1))
     out = case.cache.decode_attention(dev(q[:1]), 8, ints([n - 1])).cpu().numpy()
     check_rows(case, q[:1], out, 8, [0], [n])
+    case = Case(rng, 8, 128, (500,))            # the same in the tiles of long chunks
+    case.k[0][400:] = 30000.0 * np.sign(rng.normal(0, 1, case.k[0][400:].shape))
+    case.v[0][400:] = 30000.0
+    case.append(400, None)
+    q = rng.normal(0, 1, (400, 32 * 128)).astype(np.float32)
+    out = run_chunks(case, q, 32, (400,), (0,)).cpu().numpy()
+    pick = [0, 127, 128, 383, 384, 399]
+    check_rows(case, q[pick], out[pick], 32, [0] * 6, [p + 1 for p in pick])
 
 
 # ---- streams and graphs ----------------------------------------------------------------
