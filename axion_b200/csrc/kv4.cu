@@ -222,7 +222,7 @@ NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int entries, int
     NarrowPlan p;
     const int64_t cols = (int64_t)rows * G;
     p.cols = cols <= 4 ? 4 : cols <= 8 ? 8 : 16;
-    const int slots = ds->sm_count * (p.cols == 4 ? 4 : p.cols == 8 ? 3 : 2);
+    const int slots = ds->sm_count * (p.cols <= 8 ? 3 : 2);
     const int64_t tiles = (cols + p.cols - 1) / p.cols * c->n_kv_heads * entries;
     // every tile starts a run where that leaves half of the runs; with the most
     // tiles a call can have (it may have fewer), this many runs are never exceeded
@@ -238,7 +238,7 @@ NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int entries, int
 
 template <int HD, int COLS>
 cudaError_t launch_narrow_cols(DeviceState* ds, const NarrowArgs& a, int ctas, cudaStream_t s) {
-    static_assert(NarrowCfg<HD, COLS>::CTAS == (COLS == 4 ? 4 : COLS == 8 ? 3 : 2), "narrow_plan");
+    static_assert(NarrowCfg<HD, COLS>::CTAS == (COLS <= 8 ? 3 : 2), "narrow_plan");
     constexpr size_t smem = NarrowCfg<HD, COLS>::SMEM;
     auto kern = kv4_attn_narrow_kernel<HD, COLS>;
     static std::atomic<int> configured[64] = {};   // by device

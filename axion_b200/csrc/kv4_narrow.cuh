@@ -52,7 +52,7 @@ constexpr int kNarrowMinPages = 24;   // pages of a run at least, where every ti
 constexpr int kNarrowMinUnits = 14;   // units of a run at least elsewhere
 constexpr int kNarrowMaxParts = 96;   // parts of a tile at most (one CTA joins them)
 constexpr int kJoinThreads = 256;
-constexpr int kNarrowTileCost = 10;   // what a tile costs beside its pages, in pages
+constexpr int kNarrowTileCost = 16;   // what a tile costs beside its pages, in pages
 constexpr int kNarrowKept = 128;      // entries kept in shared memory (else read again)
 
 struct Kv4Pages {
@@ -278,7 +278,7 @@ struct NarrowCfg {
     static constexpr size_t BAR = KEPT + kNarrowKept * sizeof(NarrowEntry);
     static constexpr size_t SMEM = BAR + kNarrowWarps * NBUF * 8;
     static constexpr int JOIN_ITEMS = COLS * HD / 4 < 64 ? COLS * HD / 4 : 64;   // 4 dims of a column each
-    static constexpr int CTAS = COLS == 4 ? 4 : COLS == 8 ? 3 : 2;   // resident per SM
+    static constexpr int CTAS = COLS <= 8 ? 3 : 2;   // resident per SM
 };
 
 // The parts of the tile that begins in run blockIdx.x, joined in page order: the
