@@ -141,7 +141,7 @@ int64_t axkv4_decode_attn_workspace(const axkv4_cache_t* c, int32_t n_rows, int3
  * row with q_pos < 0 attends to nothing and gives zeros (padding of a batch).
  * Pages whose id is outside the pool count as masked and are reported in the
  * status word, as are sequences and positions outside the table.  n_heads a
- * multiple of n_kv_heads, at most 16 times as many.  The workspace's
+ * multiple of n_kv_heads, at most 16 times as many; at most 2^20 rows.  The workspace's
  * contents need not be set; calls sharing it must not overlap on the GPU. */
 int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_t n_rows,
                       int32_t n_heads, const int32_t* q_seq, const int32_t* q_pos, float* out,
@@ -156,8 +156,9 @@ int64_t axkv4_chunk_attn_workspace(const axkv4_cache_t* c, int32_t n_chunks, int
  * q_start[i + 1] - 1 of q are sequence q_seq[i] (q_seq null: sequence i) at
  * positions q_pos[i], q_pos[i] + 1, ...; each attends to tokens 0 .. its
  * position, their K and V already appended.  q_start (n_chunks + 1 device
- * int32) does not decrease; a chunk has at most max_rows rows.  q and out have
- * n_rows rows; rows of no chunk are left as they are in out.  Rows at negative
+ * int32) does not decrease; a chunk has at most max_rows rows (one that has
+ * more, or rows outside q, is left out and reported).  At most 65535 chunks of
+ * 2^24 rows.  q and out have n_rows rows; rows of no chunk are left as they are in out.  Rows at negative
  * positions give zeros; reports as in axkv4_decode_attn. */
 int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_t n_rows,
                      int32_t n_chunks, int32_t max_rows, int32_t n_heads, const int32_t* q_seq,

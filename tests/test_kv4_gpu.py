@@ -219,6 +219,44 @@ def test_decode_rows_of_chosen_sequences_and_positions():
     assert not out[4].any() and not out[6].any() and status() == 0
 
 
+@pytest.mark.parametrize("hd,heads,kv,rows", [(128, 8, 2, 300), (64, 14, 2, 129), (128, 32, 2, 140), (64, 4, 4, 128)])
+def test_decode_of_many_rows(hd, heads, kv, rows):
+    """More tiles than CTAs: runs that end inside tiles, several tiles to a run, more entries than
+    are kept in shared memory; empty rows among them."""
+    rng = np.random.default_rng(rows)
+    case = Case(rng, kv, hd, (700, 2, 129, 1500, 16))
+    seqs = rng.integers(0, 5, rows)
+    ctx = np.array([int(rng.integers(0, case.lens[s] + 1)) for s in seqs])
+    ctx[:5], seqs[:5] = case.lens, range(5)
+    q = rng.normal(0, 1, (rows, heads * hd)).astype(np.float32)
+    args = (dev(q), heads, ints(ctx - 1), ints(seqs))
+    out = case.cache.decode_attention(*args)
+    pick = sorted({0, 1, 2, 3, 4, rows // 2, rows - 2, rows - 1} | set(rng.integers(0, rows, 24).tolist()))
+    check_rows(case, q[pick], out.cpu().numpy()[pick], heads, seqs[pick], ctx[pick])
+    assert not out[torch.from_numpy(ctx == 0).cuda()].any()
+    assert torch.equal(out, case.cache.decode_attention(*args)) and status() == 0
+
+
+def test_empty_calls_and_other_types():
+    from axion_b200.kv_pages import KVPages
+    rng = np.random.default_rng(16)
+    case = Case(rng, 2, 64, (40, 20))
+    none, rows = ints([]), torch.zeros(0, 128, device="cuda")
+    case.cache.append_rows(rows, rows, none, none)
+    assert [tuple(x.shape) for x in case.cache.read_rows(none, none)] == [(0, 128), (0, 128)]
+    q = torch.zeros(0, 256, device="cuda")
+    assert case.cache.decode_attention(q, 4, none).shape == (0, 256)
+    assert case.cache.chunk_attention(q, 4, ints([0]), none, 0).shape == (0, 256)
+    pages = KVPages.empty([torch.zeros(4, 16, device="cuda")], 2, 2)
+    pages.reserve(none, none), pages.fork(none, none, none), pages.free(none), pages.copy(none, none)
+    assert int(pages.compact()) == 0 and status() == 0
+    # 16-bit queries are taken as the fp32 numbers they are
+    q16 = torch.from_numpy(rng.normal(0, 1, (2, 256)).astype(np.float16)).cuda()
+    out = case.cache.decode_attention(q16, 4, ints([39, 19]))
+    assert out.dtype == torch.float32
+    check_rows(case, q16.float().cpu().numpy(), out.cpu().numpy(), 4, [0, 1], [40, 20])
+
+
 def test_decode_long_context_keeps_its_ends():
     """20,011 tokens: the first and last token carry most of the weight, the slot behind the
     last would carry all of it, so a token lost or gained at either end shows."""
