@@ -50,7 +50,7 @@ struct Kv4Lane {
 };
 
 // Bound: HBM (4 + 0.5625 bytes a value); one read of the rows, all in registers.
-// 4095 rows of 8 x 128: 21.8 us for 38 MB, 0.27 of the copy bandwidth, at 0.74 of
+// 4095 rows of 8 x 128: 20.7 us for 38 MB, 0.28 of the copy bandwidth, at 0.75 of
 // the issue slots (rounding and packing); a warp per row and 32 dims took 38 us.
 template <int HD>
 __global__ void __launch_bounds__(256)
@@ -88,16 +88,16 @@ __global__ void __launch_bounds__(256)
         }
         const int code = kv4_step_code(hi - lo);
         const float d = code ? kv4_step(code) : 1.0f;   // all zero: any step does
-        const float inv = 1.0f / d;
+        const float inv = kv4_inverse(d);
         const float z = -kv4_round(lo, d, inv);
         uint32_t q = 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) q |= (uint32_t)fminf(kv4_round(x[e], d, inv) + z, 15.0f) << (4 * e);
+        for (int e = 0; e < 4; e++) q |= kv4_whole(fminf(kv4_round(x[e], d, inv) + z, 15.0f)) << (4 * e);
         const uint32_t other = __shfl_xor_sync(0xffffffffu, q, 2);
         if (!base) continue;
         if (i % 8 == 0)
             *reinterpret_cast<uint16_t*>(base + (kv ? F::VS : F::KS) + F::scale(slot, at.b)) =
-                (uint16_t)((code << 4) | (int)z);
+                (uint16_t)((code << 4) | kv4_whole(z));
         if (kv == 0) {
             *reinterpret_cast<uint16_t*>(base + at.k(slot)) = (uint16_t)q;
         } else {

@@ -50,15 +50,26 @@ __device__ __forceinline__ int kv4_step_code(float R) {
     return c;
 }
 
-// floor(x / d + 1/2), exactly: the product with 1/d is at most one off, and
-// the remainder x - n d of a value near a border is an fp32 number.
+// 1/d to a unit or so in the last place: kv4_round needs no more.
+__device__ __forceinline__ float kv4_inverse(float d) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return r;
+}
+
+// floor(x / d + 1/2), exactly: the product with 1/d, rounded to a whole number by
+// the addition of 1.5 * 2^23, is at most one off, and the remainder x - n d of a
+// value near a border is an fp32 number.
 __device__ __forceinline__ float kv4_round(float x, float d, float inv) {
-    float n = rintf(x * inv);
+    float n = fmaf(x, inv, 12582912.0f) - 12582912.0f;
     const float r = fmaf(-n, d, x);
     if (r >= 0.5f * d) n += 1.0f;
     if (r < -0.5f * d) n -= 1.0f;
     return n;
 }
+
+// A whole number of 0 .. 15 as an integer.
+__device__ __forceinline__ uint32_t kv4_whole(float n) { return __float_as_uint(n + 8388608.0f) & 15u; }
 
 __device__ __forceinline__ float kv4_clean(float x, bool& bad) {
     if (!(fabsf(x) <= kKv4Limit)) {
