@@ -22,12 +22,13 @@
 // the place of S in TMEM, 32 tokens at a time, in one pass: the softmax
 // reference (base 2, a whole number) moves only when a score exceeds it by more
 // than 8, and then O and the step's earlier P are multiplied by a power of two.
-// O rows go out through shared memory.
+// O rows go out through shared memory.  Every kWideKeep steps O is added to an fp32 sum
+// (kept where the rows of the output will stand) and starts anew.
 //
 // Bound: 4 x 128 x 128 x HD multiply-adds a step and tile, 5.2k cycles a step at
 // HD 128; a step takes 8.4k (a tile's softmax and products follow one another)
 // and a CTA 27k beside its steps.  Four prompts of 2048 tokens (32 query, 8 KV
-// heads of 128): 430 us, 320 TFLOP/s of the algorithm's operations, tensor cores
+// heads of 128): 466 us, 295 TFLOP/s of the algorithm's operations, tensor cores
 // busy 0.44 of the time.  Every wait is bounded; a role that gives up raises a
 // flag, and all stop.
 #pragma once
@@ -46,6 +47,11 @@ namespace axq8 {
 
 constexpr int kWideTok = 128;                      // tokens of a step
 constexpr int kWidePages = kWideTok / kKv4Tokens;
+// Steps summed in TMEM at a time.  The tensor cores' sums drop what lies below their
+// last place, always the same way: over 16,000 tokens of values of one sign an O summed
+// throughout was 1.2e-4 off, 16 steps at a time 1.3e-5, 8 below 1e-5 (values of both
+// signs: 3.8e-5, 4.9e-6, 2.7e-6).  The fp32 sums of these pieces cost 4 us each.
+constexpr int kWideKeep = 8;
 constexpr int kWideThreads = 20 * 32;              // five warpgroups, the last one for the products
 // Registers of a thread by role (setmaxnreg); at launch each has 96.
 constexpr int kWideRegs = 96, kWideRegsSoft = 128, kWideRegsTiles = 80, kWideRegsMma = 64;
@@ -206,6 +212,58 @@ __device__ __noinline__ void wide_rescale(int n16, uint32_t o, int pages, uint32
     tmem_wait_st();
 }
 
+// O of the last steps plus f times the row's sum so far (`kept`: there is one) goes to
+// memory, or (`back`) to O for the end.  A sum rests where the warp's rows of the output
+// come to stand; with 32 rows, chunk c of every lane's row side by side in row c, so
+// that a warp's access is 512 bytes in one piece.  A lane reads what itself wrote.
+template <int HD>
+__device__ __noinline__ void wide_keep(uint32_t o, float* out, int64_t row, bool live, bool kept, bool back, float f) {
+    constexpr int OL = HD / 4;
+    const int lane = threadIdx.x & 31;
+    const bool full = __all_sync(0xffffffffu, live);
+    uint32_t v[16];
+#pragma unroll 1
+    for (int c = 0; c < HD / 16; c++) {
+        float4* at[4];
+        float4 was[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int ch = 4 * c + e;
+            const int64_t r = __shfl_sync(0xffffffffu, row, full ? ch * (32 / OL) + lane / OL : lane);
+            at[e] = reinterpret_cast<float4*>(out + r) + (full ? lane % OL : ch);
+            was[e] = live && kept ? *at[e] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        tmem_ld16(o + 16 * c, v);
+        tmem_wait_ld16(v);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            was[e].x = fmaf(was[e].x, f, __uint_as_float(v[4 * e]));
+            was[e].y = fmaf(was[e].y, f, __uint_as_float(v[4 * e + 1]));
+            was[e].z = fmaf(was[e].z, f, __uint_as_float(v[4 * e + 2]));
+            was[e].w = fmaf(was[e].w, f, __uint_as_float(v[4 * e + 3]));
+        }
+        if (back) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[4 * e] = __float_as_uint(was[e].x);
+                v[4 * e + 1] = __float_as_uint(was[e].y);
+                v[4 * e + 2] = __float_as_uint(was[e].z);
+                v[4 * e + 3] = __float_as_uint(was[e].w);
+            }
+            tmem_st16(o + 16 * c, v);
+        } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) *at[e] = was[e];
+        }
+    }
+    if (back) tmem_wait_st();
+}
+
+// 2^(from - to) for two references, at least 2^-120; 2^-120 too where one is infinite.
+__device__ __forceinline__ float wide_down(float from, float to) {
+    return __uint_as_float((uint32_t)(127 + (int)fmaxf(from - to, -120.0f)) << 23);
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __grid_constant__ WideArgs a) {
     using F = Kv4<HD>;
@@ -314,12 +372,19 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
             const int pos = live && seq_ok ? min(pos0 + j, room - 1) : -1;   // the last token seen
             const int sees = __reduce_min_sync(0xffffffffu, live ? pos : 0x7fffffff);
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * C::TILE_COLS, to = ts + 128;
+            const int64_t oat = (int64_t)(r0 + j) * a.n_heads * HD + (int64_t)(kvh * a.G + min(m, rows - 1) - j * a.G) * HD;
             float base = -CUDART_INF_F, l[2] = {0.0f, 0.0f};
+            float kept = -CUDART_INF_F;   // the reference of the sum in `out`
             uint32_t s[2][32];   // 32 tokens each, the next ones on their way
             for (int st = 0; st < steps; st++) {
                 if (!lost) lost = !wide_wait(sfull + x, st & 1, stop, a.status);
                 __syncwarp();
                 tc_fence_after();
+                const bool fresh = st % kWideKeep == 0;   // O starts from zero in this step
+                if (fresh && st) {
+                    wide_keep<HD>(to, a.out, oat, live, st > kWideKeep, false, wide_down(kept, base));
+                    kept = base;
+                }
                 tmem_ld32(ts, s[0]);
                 const int tok0 = st * kWideTok;
                 const uint32_t pages = present[st & 1];
@@ -351,7 +416,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                         l[1] *= f;
                         // what is on its way has to arrive before its registers can be moved
                         if (c + 1 < kWideTok / 32) tmem_wait_ld32(s[(c + 1) & 1]);
-                        if (st || c) wide_rescale(st ? HD / 16 : 0, to, 2 * c, ts, down, f);
+                        if (!fresh || c) wide_rescale(fresh ? 0 : HD / 16, to, 2 * c, ts, down, f);
                     }
                     const float b7 = base == -CUDART_INF_F ? 0.0f : base - 7.0f;
 #pragma unroll
@@ -377,6 +442,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
             if (!lost) lost = !wide_wait(odone + x, 0, stop, a.status);
             __syncwarp();
             tc_fence_after();
+            if (steps > kWideKeep) wide_keep<HD>(to, a.out, oat, live, true, true, wide_down(kept, base));
             const float sum = l[0] + l[1];
             const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;   // nothing seen: zeros
             uint8_t* orow = sm + (128 * x + r) * C::OROW;
@@ -393,7 +459,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
             __syncwarp();
             // this warp's rows, HD / 4 lanes to a row
             constexpr int OL = HD / 4;
-            const int64_t oat = (int64_t)(r0 + j) * a.n_heads * HD + (int64_t)(kvh * a.G + min(m, rows - 1) - j * a.G) * HD;
 #pragma unroll 4
             for (int k = 0; k < OL; k++) {
                 const int rr = k * (32 / OL) + lane / OL;
@@ -576,7 +641,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                 for (int p = 0; p < kWidePages; p++) {
                     const uint64_t vd = sw128_kmajor_desc(va + (p / 4) * C::VATOM) + 2 * (p & 3);
                     mma_f16_ts(d, tmem + x * C::TILE_COLS + (p / 2) * 32 + (1 - part) * 16 + (p & 1) * 8, vd, ipv,
-                               st | part | p);
+                               st % kWideKeep | part | p);
                 }
         };
         bool ok = wide_wait(qfull, 0, stop, a.status) && wide_wait(kfull, 0, stop, a.status);

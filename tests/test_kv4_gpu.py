@@ -419,6 +419,33 @@ def test_chunk_attention_of_long_chunks(hd, heads, kv, rows, past):
     assert torch.equal(out, first)                   # bit for bit
 
 
+@pytest.mark.parametrize("heads,hd,kv,rows,past", [(32, 128, 8, 200, 16000), (16, 64, 8, 330, 7000)])
+def test_long_chunks_over_a_long_past(heads, hd, kv, rows, past):
+    """Sums of values of one sign over thousands of tokens: what the tensor cores drop at each of
+    their sums (at most a unit in the last place, always the same way) must not pile up.  1024
+    tokens summed there take 128 products, each dropping at most 2^-23 of a sum that grows
+    evenly: 128 / 2 * 2^-23 = 7.6e-6; the rest (weights kept to 2^-22, partial sums added in
+    fp32) is below 2e-6."""
+    rng = np.random.default_rng(past)
+    case = Case(rng, kv, hd, (past + rows,))
+    case.v[0][:] = np.abs(case.v[0]) + 0.5
+    case.append(0, None)
+    q = rng.normal(0, 1, (rows, heads * hd)).astype(np.float32)
+    out = run_chunks(case, q, heads, (rows,), (past,))
+    assert torch.equal(out, run_chunks(case, q, heads, (rows,), (past,)))
+    out, worst = out.cpu().numpy(), 0.0
+    for kvh in range(kv):
+        k, v = case.held(0, past + rows, kvh)
+        h = kvh * (heads // kv)
+        for r in (0, rows // 2, rows - 1):
+            n = past + r + 1
+            ref = km.attention(q[r].reshape(heads, hd)[h].astype(np.float64), k[:n], v[:n], 1 / np.sqrt(hd))
+            err = np.linalg.norm(out[r].reshape(heads, hd)[h] - ref) / np.linalg.norm(ref)
+            worst = max(worst, err)
+    assert worst <= 1e-5, worst
+    assert status() == 0
+
+
 def test_long_chunks_with_empty_rows_and_bad_pages():
     """Positions before the start, a page outside the pool, a sequence outside the table."""
     from axion_b200 import _lib
