@@ -323,12 +323,12 @@ cudaError_t launch_wide(DeviceState* ds, const axkv4_cache_t* c, const float* q,
 
 // Whether the tensor-core tiles of 256 rows (kv4_wide.cuh) take a chunk call, or the
 // column tiles of 16 (kv4_narrow.cuh), which share a long context among all SMs.
-// Measured per page of context: a CTA of the first takes 0.58 us, whatever its
+// Measured per page of context: a CTA of the first takes 0.61 us, whatever its
 // rows, one to an SM; a tile of the second 0.27 us of an SM.
 bool wide_takes(DeviceState* ds, const axkv4_cache_t* c, int chunks, int rows, int G) {
     const int64_t cols = (int64_t)rows * G, lists = (int64_t)chunks * c->n_kv_heads;
     const int64_t waves = (lists * ((cols + 255) / 256) + ds->sm_count - 1) / ds->sm_count;
-    return 58 * waves * ds->sm_count < 27 * lists * ((cols + 15) / 16);
+    return 61 * waves * ds->sm_count < 27 * lists * ((cols + 15) / 16);
 }
 
 }  // namespace
