@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_attn_join_kernel(const __gri
     float mx = -CUDART_INF_F, sum = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     auto add = [&](float2 ml, float4 x) {
-        if (ml.x == -CUDART_INF_F) return;
+        if (ml.x == -CUDART_INF_F && ml.y == 0.0f) return;   // saw nothing (a NaN query: sum NaN, which stays)
         const float m = fmaxf(mx, ml.x), f = ex2(mx - m), h = ex2(ml.x - m);
         mx = m;
         v.x = fmaf(v.x, f, x.x * h);
