@@ -5,7 +5,8 @@ of any number of layers and moves page contents in every layer's pool: the
 ``k`` and ``v`` tensors of :class:`~axion_b200.paged_kv.PagedKVCache`-like fp16
 or fp32 pages, or the ``pages`` of :class:`~axion_b200.paged_kv.PagedKVCache4`.
 Everything stays on the device: no call synchronizes or reads back, so serving
-loops can capture them.  Invalid entries and a pool without enough free pages
+loops can capture them.  Threads may share a table on one stream: a call's
+kernels are launched together.  Invalid entries and a pool without enough free pages
 are reported in the device status word (``ops.status()``); such a reserve or
 fork changes nothing.
 """
@@ -88,7 +89,7 @@ class KVPages(_DeviceCalls):
     def free(self, seqs: torch.Tensor) -> None:
         """Sequences give their pages up."""
         n, at = self._list(seqs)
-        self._call(self._lib.axkv_pages_free, *at, n)
+        self._call_alone(self._lib.axkv_pages_free, *at, n)
 
     def compact(self) -> torch.Tensor:
         """Live pages to the front of every pool; their number (int32 [1])."""
@@ -99,4 +100,4 @@ class KVPages(_DeviceCalls):
     def copy(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Page src[i] to page dst[i] in every pool (no destination twice, none a source)."""
         n, at = self._list(src, dst)
-        self._call(self._lib.axkv_pages_copy, *at, n)
+        self._call_alone(self._lib.axkv_pages_copy, *at, n)

@@ -163,6 +163,11 @@ class _DeviceCalls:
         if rc:
             check(rc)
 
+    def _call_alone(self, fn, *args) -> None:
+        """_call, not between the kernels of another thread's call."""
+        with self._lock:
+            self._call(fn, *args)
+
     def _call_ws(self, need: int, fn, *args) -> None:
         """_call with a workspace of `need` bytes: kept per stream, on which calls
         follow one another (the kernels of a call too: threads take turns); a

@@ -176,7 +176,8 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
  * pages to allocate than are free, changes nothing and is reported in the
  * status word (AXQ8_ERR_INVALID, AXQ8_ERR_ALLOC); a free or copy leaves
  * invalid entries out and reports them.  Calls on one state must not overlap
- * on the GPU. */
+ * on the GPU, and come from one host thread at a time: a reserve, fork or compact
+ * is two kernels, between which no other call on the state may be launched. */
 typedef struct axkv_pages {
     int32_t* block_table;        /* device [n_seqs][max_blocks] */
     int32_t* ref_count;          /* device [n_pages] */
