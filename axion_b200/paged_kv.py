@@ -172,6 +172,9 @@ class _DeviceCalls:
         """_call with a workspace of `need` bytes: kept per stream, on which calls
         follow one another (the kernels of a call too: threads take turns); a
         captured graph's is its own."""
+        if torch._C._cuda_getDevice() != self._dev:   # capture is asked of the current device
+            with torch.cuda.device(self._device):
+                return self._call_ws(need, fn, *args)
         if torch.cuda.is_current_stream_capturing():
             ws = torch.empty(need, dtype=torch.uint8, device=self._device)
             return self._call(fn, *args, ws.data_ptr(), need)
