@@ -156,6 +156,7 @@ int check_cache4(const axkv4_cache_t* c, const char* what) {
         return fail(AXQ8_ERR_UNSUPPORTED, "%s: head_dim %d (32, 64, 128)", what, c->head_dim);
     if (c->n_seqs <= 0 || c->n_pages <= 0 || c->max_blocks <= 0 || c->n_kv_heads <= 0)
         return fail(AXQ8_ERR_INVALID, "%s: non-positive cache dimension", what);
+    if (c->n_kv_heads > 65535) return fail(AXQ8_ERR_UNSUPPORTED, "%s: %d KV heads", what, c->n_kv_heads);
     if (c->max_blocks > (1 << 26)) return fail(AXQ8_ERR_UNSUPPORTED, "%s: max_blocks %d", what, c->max_blocks);
     if (reinterpret_cast<uintptr_t>(c->pages) & 15)
         return fail(AXQ8_ERR_INVALID, "%s: pages not 16-byte aligned", what);
@@ -213,18 +214,45 @@ cudaError_t launch_read(const axkv4_cache_t* c, float* k, float* v, int64_t ld, 
                     pages_of(c), k, v, ld, n_rows, seq, pos, status);
 }
 
+int narrow_cols(int64_t cols) { return cols <= 4 ? 4 : cols <= 8 ? 8 : 16; }
+
+// Whether the column tiles' units of work (runs of them rounded up: at most twice as
+// many) count in 32 bits.
+int check_narrow(const axkv4_cache_t* c, const char* what, int entries, int rows, int G) {
+    const int64_t cols = (int64_t)rows * G, per = narrow_cols(cols);
+    const double tiles = (double)((cols + per - 1) / per) * c->n_kv_heads * entries;
+    if (tiles * (c->max_blocks + kNarrowTileCost) * 2 > 2147483647.0)
+        return fail(AXQ8_ERR_UNSUPPORTED, "%s: %d chunks of at most %d rows over %d pages", what, entries, rows,
+                    c->max_blocks);
+    return AXQ8_OK;
+}
+
+int check_decode(const axkv4_cache_t* c, const char* what, int32_t n_rows, int32_t n_heads) {
+    const int rc = check_attn(c, what, n_heads);
+    if (rc) return rc;
+    if (n_rows < 0 || n_rows > (1 << 20)) return fail(AXQ8_ERR_INVALID, "%s: n_rows %d", what, n_rows);
+    return check_narrow(c, what, n_rows, 1, n_heads / c->n_kv_heads);
+}
+
+int check_chunks(const axkv4_cache_t* c, const char* what, int32_t n_chunks, int32_t max_rows, int32_t n_heads) {
+    const int rc = check_attn(c, what, n_heads);
+    if (rc) return rc;
+    if (n_chunks < 0 || max_rows < 0 || n_chunks > 65535 || max_rows > (1 << 24))
+        return fail(AXQ8_ERR_INVALID, "%s: %d chunks of at most %d rows", what, n_chunks, max_rows);
+    return AXQ8_OK;
+}
+
 // Columns of a tile, CTAs, and workspace bytes: a record per CTA, then two
 // partial states per CTA.
 struct NarrowPlan {
     int cols, ctas, aligned;
     int64_t records, workspace;
-    int64_t units;   // of work, at most
 };
 
 NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int entries, int rows, int G) {
     NarrowPlan p;
     const int64_t cols = (int64_t)rows * G;
-    p.cols = cols <= 4 ? 4 : cols <= 8 ? 8 : 16;
+    p.cols = narrow_cols(cols);
     const int slots = ds->sm_count * (p.cols <= 8 ? 3 : 2);
     const int64_t tiles = (cols + p.cols - 1) / p.cols * c->n_kv_heads * entries;
     // every tile starts a run where that leaves half of the runs; with the most
@@ -233,7 +261,6 @@ NarrowPlan narrow_plan(DeviceState* ds, const axkv4_cache_t* c, int entries, int
     const int64_t runs = p.aligned ? (tiles * c->max_blocks + kNarrowMinPages - 1) / kNarrowMinPages + p.aligned
                                    : (tiles * (c->max_blocks + kNarrowTileCost) + kNarrowMinUnits - 1) / kNarrowMinUnits;
     p.ctas = (int)std::min<int64_t>(slots, runs);
-    p.units = tiles * (c->max_blocks + kNarrowTileCost) * 2;
     p.records = ((int64_t)p.ctas * sizeof(NarrowPart) + 15) / 16 * 16;
     p.workspace = p.records + (int64_t)p.ctas * 2 * p.cols * (c->head_dim + 2) * 4;
     return p;
@@ -365,7 +392,7 @@ int axkv4_read(const axkv4_cache_t* c, float* k_rows, float* v_rows, int64_t ld,
 }
 
 int64_t axkv4_decode_attn_workspace(const axkv4_cache_t* c, int32_t n_rows, int32_t n_heads) {
-    if (check_attn(c, "axkv4_decode_attn_workspace", n_heads) || n_rows <= 0) return -1;
+    if (check_decode(c, "axkv4_decode_attn_workspace", n_rows, n_heads) || n_rows == 0) return -1;
     DeviceState* ds = device_state();
     if (!ds) return -1;
     return narrow_plan(ds, c, n_rows, 1, n_heads / c->n_kv_heads).workspace;
@@ -374,9 +401,8 @@ int64_t axkv4_decode_attn_workspace(const axkv4_cache_t* c, int32_t n_rows, int3
 int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_t n_rows,
                       int32_t n_heads, const int32_t* q_seq, const int32_t* q_pos, float* out,
                       void* workspace, int64_t workspace_bytes, void* stream) {
-    int rc = check_attn(c, "axkv4_decode_attn", n_heads);
+    int rc = check_decode(c, "axkv4_decode_attn", n_rows, n_heads);
     if (rc) return rc;
-    if (n_rows < 0 || n_rows > (1 << 20)) return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: n_rows %d", n_rows);
     if (n_rows == 0) return AXQ8_OK;
     if (!q || !q_pos || !out || !workspace) return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: null pointer");
     if (ldq < (int64_t)n_heads * c->head_dim || ldq % 4 ||
@@ -389,8 +415,6 @@ int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
     const NarrowPlan p = narrow_plan(ds, c, n_rows, 1, n_heads / c->n_kv_heads);
-    if (p.units > 0x7fffffff)
-        return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_decode_attn: %d rows of %d pages", n_rows, c->max_blocks);
     if (workspace_bytes < p.workspace)
         return fail(AXQ8_ERR_INVALID, "axkv4_decode_attn: workspace %lld B < %lld B",
                     (long long)workspace_bytes, (long long)p.workspace);
@@ -402,10 +426,12 @@ int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32
 
 int64_t axkv4_chunk_attn_workspace(const axkv4_cache_t* c, int32_t n_chunks, int32_t max_rows,
                                    int32_t n_heads) {
-    if (check_attn(c, "axkv4_chunk_attn_workspace", n_heads) || n_chunks <= 0 || max_rows <= 0) return -1;
+    if (check_chunks(c, "axkv4_chunk_attn_workspace", n_chunks, max_rows, n_heads) || n_chunks == 0 || max_rows == 0)
+        return -1;
     DeviceState* ds = device_state();
     if (!ds) return -1;
     if (wide_takes(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads)) return 16;
+    if (check_narrow(c, "axkv4_chunk_attn_workspace", n_chunks, max_rows, n_heads / c->n_kv_heads)) return -1;
     return narrow_plan(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads).workspace;
 }
 
@@ -413,11 +439,9 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
                      int32_t n_chunks, int32_t max_rows, int32_t n_heads, const int32_t* q_seq,
                      const int32_t* q_start, const int32_t* q_pos, float* out, void* workspace,
                      int64_t workspace_bytes, void* stream) {
-    int rc = check_attn(c, "axkv4_chunk_attn", n_heads);
+    int rc = check_chunks(c, "axkv4_chunk_attn", n_chunks, max_rows, n_heads);
     if (rc) return rc;
-    if (n_rows < 0 || n_chunks < 0 || max_rows < 0 || n_chunks > 65535 || max_rows > (1 << 24))
-        return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: %d rows, %d chunks of at most %d", n_rows, n_chunks,
-                    max_rows);
+    if (n_rows < 0) return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: %d rows", n_rows);
     if (n_rows == 0 || n_chunks == 0 || max_rows == 0) return AXQ8_OK;
     if (!q || !q_start || !q_pos || !out || !workspace)
         return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: null pointer");
@@ -431,17 +455,14 @@ int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_
     DeviceState* ds = device_state();
     if (!ds) return AXQ8_ERR_CUDA;
     if (wide_takes(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads)) {
-        if (c->n_kv_heads > 65535) return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d KV heads", c->n_kv_heads);
         AXQ8_CUDA_TRY(KV4_BY_HEAD_DIM(c->head_dim, launch_wide, ds, c, q, ldq, n_rows, n_chunks, max_rows, n_heads,
                                       q_seq, q_start, q_pos, out,
                                       static_cast<cudaStream_t>(stream)),
                       "axkv4_chunk_attn launch");
         return AXQ8_OK;
     }
+    if ((rc = check_narrow(c, "axkv4_chunk_attn", n_chunks, max_rows, n_heads / c->n_kv_heads))) return rc;
     const NarrowPlan p = narrow_plan(ds, c, n_chunks, max_rows, n_heads / c->n_kv_heads);
-    if (p.units > 0x7fffffff)
-        return fail(AXQ8_ERR_UNSUPPORTED, "axkv4_chunk_attn: %d chunks of %d rows, %d pages", n_chunks,
-                    max_rows, c->max_blocks);
     if (workspace_bytes < p.workspace)
         return fail(AXQ8_ERR_INVALID, "axkv4_chunk_attn: workspace %lld B < %lld B",
                     (long long)workspace_bytes, (long long)p.workspace);

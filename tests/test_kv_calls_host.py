@@ -1,6 +1,7 @@
 """Host side of the 4-bit cache's and the page table's calls, without a GPU."""
 from __future__ import annotations
 
+import ctypes as C
 import threading
 
 import pytest
@@ -65,3 +66,28 @@ def test_a_workspace_is_a_graphs_own_where_the_objects_stream_is_captured(calls,
     Devices.capturing = {0}                       # the other device's capture is none of ours
     calls._call_ws(64, fn)
     assert list(calls._ws) == [101] and Devices.current == current
+
+
+@pytest.mark.parametrize("max_blocks,n_kv,rows,heads,word", [
+    (4, 2, (1 << 20) + 1, 4, b"n_rows"), (4, 2, -1, 4, b"n_rows"), (1 << 26, 2, 8, 4, b"pages"),
+    (1 << 20, 8, 1 << 10, 32, b"pages"), (4, 1 << 16, 1, 1 << 16, b"KV heads")])
+def test_a_workspace_is_refused_where_the_decode_call_is(max_blocks, n_kv, rows, heads, word):
+    """Both answer alike, before any work on a device."""
+    from axion_b200 import _lib
+    lib = _lib.load()
+    c = C.byref(_lib.axkv4_cache_t(4096, 4096, 1 << 21, max_blocks, 8, n_kv, 64, 16))
+    assert lib.axkv4_decode_attn_workspace(c, rows, heads) == -1
+    assert word in lib.axq8_last_error() and b"workspace" in lib.axq8_last_error()
+    rc = lib.axkv4_decode_attn(c, 4096, heads * 64, rows, heads, None, 4096, 4096, 4096, 1 << 40, None)
+    assert rc in (_lib.AXQ8_ERR_INVALID, _lib.AXQ8_ERR_UNSUPPORTED) and word in lib.axq8_last_error()
+
+
+@pytest.mark.parametrize("chunks,rows", [(65536, 1), (1, (1 << 24) + 1), (-1, 1), (1, -1)])
+def test_a_workspace_is_refused_where_the_chunk_call_is(chunks, rows):
+    from axion_b200 import _lib
+    lib = _lib.load()
+    c = C.byref(_lib.axkv4_cache_t(4096, 4096, 1 << 17, 4, 8, 2, 64, 16))
+    assert lib.axkv4_chunk_attn_workspace(c, chunks, rows, 4) == -1
+    assert b"chunks of at most" in lib.axq8_last_error()
+    assert lib.axkv4_chunk_attn(c, 4096, 256, 8, chunks, rows, 4, None, 4096, 4096, 4096, 4096, 1 << 40,
+                                None) == _lib.AXQ8_ERR_INVALID
