@@ -50,7 +50,7 @@ constexpr int kWidePages = kWideTok / kKv4Tokens;
 // Steps summed in TMEM at a time.  The tensor cores' sums drop what lies below their
 // last place, always the same way: over 16,000 tokens of values of one sign an O summed
 // throughout was 1.2e-4 off, 16 steps at a time 1.3e-5, 8 below 1e-5 (values of both
-// signs: 3.8e-5, 4.9e-6, 2.7e-6).  The fp32 sums of these pieces cost 4 us each.
+// signs: 3.8e-5, 4.9e-6, 2.7e-6; all tokens alike: 8 at most 2.1e-5).  The fp32 sums of these pieces cost 4 us each.
 constexpr int kWideKeep = 8;
 constexpr int kWideThreads = 20 * 32;              // five warpgroups, the last one for the products
 // Registers of a thread by role (setmaxnreg); at launch each has 96.
@@ -373,7 +373,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
             const int sees = __reduce_min_sync(0xffffffffu, live ? pos : 0x7fffffff);
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * C::TILE_COLS, to = ts + 128;
             const int64_t oat = (int64_t)(r0 + j) * a.n_heads * HD + (int64_t)(kvh * a.G + min(m, rows - 1) - j * a.G) * HD;
-            float base = -CUDART_INF_F, l[2] = {0.0f, 0.0f};
+            // the weights' sum and what its additions lost (equal weights lose the same at each: a
+            // plain sum was 1.2e-4 off at 16,000 tokens), and the sum of a step
+            float base = -CUDART_INF_F, l = 0.0f, l_lost = 0.0f, l_step[2] = {0.0f, 0.0f};
             float kept = -CUDART_INF_F;   // the reference of the sum in `out`
             uint32_t s[2][32];   // 32 tokens each, the next ones on their way
             for (int st = 0; st < steps; st++) {
@@ -412,8 +414,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                         const int down = over && base != -CUDART_INF_F ? (int)fmaxf(base - to_base, -120.0f) : 0;
                         base = to_base;
                         const float f = __uint_as_float((uint32_t)(127 + down) << 23);
-                        l[0] *= f;
-                        l[1] *= f;
+                        l *= f;
+                        l_lost *= f;
+                        l_step[0] *= f;
+                        l_step[1] *= f;
                         // what is on its way has to arrive before its registers can be moved
                         if (c + 1 < kWideTok / 32) tmem_wait_ld32(s[(c + 1) & 1]);
                         if (!fresh || c) wide_rescale(fresh ? 0 : HD / 16, to, 2 * c, ts, down, f);
@@ -426,8 +430,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                         for (int e = 0; e < 8; e++) {
                             const float w0 = ex2(fmaf(__uint_as_float(v[16 * p + 2 * e]), mul, -b7));
                             const float w1 = ex2(fmaf(__uint_as_float(v[16 * p + 2 * e + 1]), mul, -b7));
-                            l[0] += w0;
-                            l[1] += w1;
+                            l_step[0] += w0;
+                            l_step[1] += w1;
                             split2(w0, w1, hi[e], lo[e]);
                         }
                         tmem_st8(ts + 32 * c + 8 * p, hi);
@@ -437,13 +441,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(pfull + x);
+                const float add = l_step[0] + l_step[1], sum = l + add, had = sum - add;
+                l_lost += (l - had) + (add - (sum - had));
+                l = sum;
+                l_step[0] = l_step[1] = 0.0f;
             }
             // O / l: the tile's rows to shared memory (Q and K are read), from there to `out`
             if (!lost) lost = !wide_wait(odone + x, 0, stop, a.status);
             __syncwarp();
             tc_fence_after();
             if (steps > kWideKeep) wide_keep<HD>(to, a.out, oat, live, true, true, wide_down(kept, base));
-            const float sum = l[0] + l[1];
+            const float sum = l + l_lost;
             const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;   // nothing seen: zeros
             uint8_t* orow = sm + (128 * x + r) * C::OROW;
 #pragma unroll

@@ -35,3 +35,32 @@ def test_a_query_that_is_no_number_shows_in_its_heads(hd, heads, kv, n):
             scale = 1 / np.sqrt(hd)
             ref = km.attention(q[0, h].astype(np.float64), k, v, scale)
             assert np.abs(out[h] - ref).max() <= km.tolerance(q[0, h].astype(np.float64), k, v, scale)
+
+
+def equal_tokens(rng, case, n):
+    """Every token of every sequence the same K and the same positive V: the result is V itself."""
+    k, v = rng.normal(0, 1, (case.kv, case.hd)), rng.uniform(0.5, 1.5, (case.kv, case.hd))
+    for s in range(len(case.lens)):
+        case.k[s][:], case.v[s][:] = k, v
+    case.append(0, None)
+    return np.stack([case.held(0, 1, h)[1][0] for h in range(case.kv)])          # [kv, hd]
+
+
+@pytest.mark.parametrize("heads,hd,kv,rows,past", [(32, 128, 8, 200, 16000), (16, 64, 8, 330, 7000)])
+def test_long_chunks_of_equal_tokens(heads, hd, kv, rows, past):
+    """Equal weights round the same way at every addition, and equal products are cut alike.
+    The weights' sum is taken 128 tokens at a time (two chains of 64 additions of at most 2^-24:
+    3.8e-6) and joined without loss.  O: a tensor core aligns the 16 products of an instruction
+    and the sum to the largest and cuts them, at least two bits below the sum's last place (as
+    measured by Fasi, Higham, Mikaitis and Pranesh, Numerical behavior of NVIDIA tensor cores,
+    2021), so 16 / 4 + 1 = 5 units of at most 2^-23 of the sum; 128 instructions are a piece of
+    1024 tokens, whose sum grows evenly: 128 / 2 * 5 * 2^-23 = 3.8e-5.  The weights' fp16 pairs
+    2.4e-7, 17 pieces of 2^-24.  (One chain of additions was 1.3e-4 and 7e-5 off here.)"""
+    rng = np.random.default_rng(past + 1)
+    case = Case(rng, kv, hd, (past + rows,))
+    v = equal_tokens(rng, case, past + rows)
+    q = rng.normal(0, 1, (rows, heads * hd)).astype(np.float32)
+    out = run_chunks(case, q, heads, (rows,), (past,)).cpu().numpy().reshape(rows, kv, -1, hd)
+    worst = np.abs(out / v[None, :, None] - 1).max()
+    assert worst <= 128 / 2 * 5 * 2.0 ** -23 + 64 * 2.0 ** -24 + 2.0 ** -22 + 17 * 2.0 ** -24, worst
+    assert status() == 0
