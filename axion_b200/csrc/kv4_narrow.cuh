@@ -12,9 +12,13 @@
 //      the integer product, in fp32.
 //   V: a nibble in place times D plus Z is (q - z) d 2^(e - 24) in one fused
 //      multiply-add, with D = d 2^e (high nibbles: d 2^(e - 4)) and Z = -z d
-//      2^(e - 24).  e is the warp's: the largest d so far becomes 2^13 to 2^16,
-//      and O is rescaled when a larger one comes.  All of it is exact for d
-//      down to 2^-7 of that, and to 2^-25 of the largest product below.
+//      2^(e - 24): exact while D is 2^6 to 2^16.  e is kept from step to step and
+//      moves when a step's d leave that window; where they are too far apart for any
+//      (a factor of 2^9: tokens or blocks of dims of very different size, or a draft
+//      row's token that the others do not see), the step forms (q - z) d by a subtraction and
+//      a product, exact for every d, at a third instruction for a pair.  O is
+//      the plain sum either way.  (One e for all tokens so far, small d rounded,
+//      measured 0.5 us less of 54 at batch 64; the second form throughout, 3.2 more.)
 // Q (scaled by a power of two to below 2^14) and P (2^7 times the softmax
 // weight) are an fp16 high part plus an fp16 residual: results keep fp32
 // accuracy.  Up to four columns, the two parts are two columns of one product
@@ -45,6 +49,8 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "decode_ops.cuh"
@@ -558,8 +564,8 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
     low = __reduce_min_sync(0xffffffffu, low);
 
     const float rest = t < 2 ? 0.0f : -1.0f;
-    int dexp = 0;           // e: O holds the sum times 2^(e - 24)
-    uint32_t dtop = 0;      // bits of the d from which e has to fall
+    int dexp = 0;                   // e, and the words of a step's scales that it takes:
+    uint32_t dlow = 0, dspan = 0;   // dlow .. dlow + dspan - 1
     float o[NT][MT][4], base[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -586,7 +592,8 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
             tok0[p] = (bad >> (PP * s + p)) & 1 ? 0x40000000
                                                 : (part_b0 + (it * W + warp) * PP + p) * kKv4Tokens;
         // V factors: lane (g, t) makes those of block b = g % NB, tokens 2t + 8u, 2t + 1 + 8u
-        uint32_t dz[PP][2], dmax = 0;
+        uint32_t dz[PP];
+        bool out = false;
 #pragma unroll
         for (int p = 0; p < PP; p++) {
             const uint8_t* vs = buf + p * F::BYTES + F::VS;
@@ -597,39 +604,43 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
                 if (tok0[p] + r >= ctx) wa = 0;
                 if (tok0[p] + r + 1 >= ctx) wb = 0;
             }
-            dmax = max(dmax, max(wa, wb));
-            const uint32_t w = __byte_perm(wa, wb, 0x5410);
-            dz[p][0] = w & 0x7ff07ff0u;
-            dz[p][1] = w & 0x000f000fu;
+            out |= wa - dlow >= dspan || wb - dlow >= dspan;
+            dz[p] = __byte_perm(wa, wb, 0x5410);
         }
-        dmax = __reduce_max_sync(0xffffffffu, dmax);   // the largest d, and some zero point
-        if (dmax >= dtop) {                            // beyond 2^16 / 2^e
-            const int ne = 28 - (int)(dmax >> 10);
-            const float f = __uint_as_float((uint32_t)(127 + ne - dexp) << 23);
-            dexp = ne;
-            dtop = (uint32_t)(31 - ne) << 10;
-            if (it) {
+        bool near = true;
+        if (__any_sync(0xffffffffu, out)) {
+            uint32_t top = 0, low = 0xffffffffu;   // the largest and the smallest d, zeros aside, and some zero point
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int k = 0; k < MT; k++) {
-                        o[n][k][0] *= f;
-                        o[n][k][1] *= f;
-                        o[n][k][2] *= f;
-                        o[n][k][3] *= f;
-                    }
+            for (int p = 0; p < PP; p++) {
+                top = max(top, max(dz[p] & 0xffffu, dz[p] >> 16));
+                low = min(low, min((dz[p] & 0xffffu) - 16u, (dz[p] >> 16) - 16u));
+            }
+            top = __reduce_max_sync(0xffffffffu, top) >> 10;
+            low = __reduce_min_sync(0xffffffffu, low) + 16u;
+            if (low >> 10 == 0 && low >= 16) near = top <= 4;   // below 2^-14: down to 2^-20
+            else near = low < 16 || top <= (low >> 10) + 9;
+            if (near) {
+                const uint32_t spare = top <= 4 ? 0 : 9 - min(9u, low < 16 ? 0 : top - (low >> 10));
+                dexp = 30 - (int)(top + spare / 2);
+                dlow = dexp >= 26 ? 16 : (uint32_t)max(1, 21 - dexp) << 10;
+                dspan = ((uint32_t)(31 - dexp) << 10) - dlow;
             }
         }
-        {
+        if (near) {
             const uint32_t up1 = f16_pow2(dexp / 2), up2 = f16_pow2(dexp - dexp / 2);
 #pragma unroll
             for (int p = 0; p < PP; p++) {
-                const uint32_t D = hmul2u(hmul2u(dz[p][0], up1), up2);
-                const uint32_t Z = hmul2u(dz[p][1], D) ^ 0x80008000u;
+                const uint32_t D = hmul2u(hmul2u(dz[p] & 0x7ff07ff0u, up1), up2);
                 if (g < 2 * NB)
                     *reinterpret_cast<uint2*>(vsc + p * C::VSC_PAGE + ((t * NB + g % NB) * 2 + g / NB) * 8) =
-                        make_uint2(D, Z);
+                        make_uint2(D, hmul2u(dz[p] & 0x000f000fu, D) ^ 0x80008000u);
             }
+        } else {
+#pragma unroll
+            for (int p = 0; p < PP; p++)
+                if (g < 2 * NB)
+                    *reinterpret_cast<uint2*>(vsc + p * C::VSC_PAGE + ((t * NB + g % NB) * 2 + g / NB) * 8) =
+                        make_uint2(dz[p] & 0x7ff07ff0u, (dz[p] & 0x000f000fu) | 0x64006400u);
         }
         // scores: tokens g (sc[..][0], [1]) and g + 8 ([2], [3]), columns tq, tq + 1
         float sc[PP][NT][4];
@@ -755,61 +766,63 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
         // largest term, so a step's products are summed from zero and added in
         // fp32: the error does not grow with the number of pages.
         constexpr int TPG = F::TPG;
-        uint32_t f2[PP][4], dh[PP][2];   // D and Z of tokens (2t, 2t + 1), (2t + 8, 2t + 9), D / 16
+        const float back = __uint_as_float((uint32_t)(127 + 24 - dexp) << 23);
+        auto add_values = [&](auto is_near) {
+            constexpr bool NEAR = decltype(is_near)::value;
+            // factors of tokens (2t, 2t + 1), (2t + 8, 2t + 9), and what high nibbles take instead
+            uint32_t f2[PP][4], fh[PP][2];
 #pragma unroll
-        for (int m0 = 0; m0 < MT; m0 += TPG) {
-            uint32_t x[PP][TPG];
+            for (int m0 = 0; m0 < MT; m0 += TPG) {
+                uint32_t x[PP][TPG];
 #pragma unroll
-            for (int p = 0; p < PP; p++)
-                lds_words<TPG>(x[p], buf + p * F::BYTES + F::V + (m0 / TPG) * (128 * TPG) + lane * (4 * TPG));
+                for (int p = 0; p < PP; p++)
+                    lds_words<TPG>(x[p], buf + p * F::BYTES + F::V + (m0 / TPG) * (128 * TPG) + lane * (4 * TPG));
 #pragma unroll
-            for (int k = 0; k < TPG; k++) {
-                const int m = m0 + k, b = m / 2;
-                float c[NT][4];
+                for (int k = 0; k < TPG; k++) {
+                    const int m = m0 + k, b = m / 2;
+                    float c[NT][4];
 #pragma unroll
-                for (int p = 0; p < PP; p++) {
-                    if (m % 2 == 0) {
-                        lds_words<4>(f2[p], vsc + p * C::VSC_PAGE + (t * NB + b) * 16);
-                        dh[p][0] = hmul2u(f2[p][0], 0x2c002c00u);
-                        dh[p][1] = hmul2u(f2[p][2], 0x2c002c00u);
-                    }
-                    uint32_t v[4];
+                    for (int p = 0; p < PP; p++) {
+                        if (m % 2 == 0) {
+                            lds_words<4>(f2[p], vsc + p * C::VSC_PAGE + (t * NB + b) * 16);
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const uint32_t y = u ? x[p][k] >> 8 : x[p][k], D = f2[p][2 * u], Z = f2[p][2 * u + 1];
-                        v[2 * u] = hfma2u(y & 0x000f000fu, D, Z);
-                        v[2 * u + 1] = hfma2u(y & 0x00f000f0u, dh[p][u], Z);
-                    }
+                            for (int u = 0; u < 2; u++)   // D / 16, or 64 + z
+                                fh[p][u] = NEAR ? hmul2u(f2[p][2 * u], 0x2c002c00u)
+                                                : (f2[p][2 * u + 1] & 0x000f000fu) * 16 + 0x54005400u;
+                        }
+                        uint32_t v[4];
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        if constexpr (PACK) {
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t y = u ? x[p][k] >> 8 : x[p][k], d = f2[p][2 * u], z = f2[p][2 * u + 1];
+                            if constexpr (NEAR) {
+                                v[2 * u] = hfma2u(y & 0x000f000fu, d, z);
+                                v[2 * u + 1] = hfma2u(y & 0x00f000f0u, fh[p][u], z);
+                            } else {
+                                v[2 * u] = hmul2u(hsub2u((y & 0x000f000fu) | 0x64006400u, z), d);
+                                v[2 * u + 1] = hmul2u(hsub2u((y & 0x00f000f0u) | 0x54005400u, fh[p][u]), d);
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
                             if (p == 0) mma_f16_16816_first(c[n], v, ph[p][n][0], ph[p][n][1]);
                             else mma_f16_16816(c[n], v, ph[p][n][0], ph[p][n][1]);
-                        } else {
-                            if (p == 0) mma_f16_16816_first(c[n], v, ph[p][n][0], ph[p][n][1]);
-                            else mma_f16_16816(c[n], v, ph[p][n][0], ph[p][n][1]);
-                            mma_f16_16816(c[n], v, pl[p][n][0], pl[p][n][1]);
+                            if constexpr (!PACK) mma_f16_16816(c[n], v, pl[p][n][0], pl[p][n][1]);
                         }
                     }
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[n][m][j] = fmaf(c[n][j], NEAR ? back : 1.0f, o[n][m][j]);
                 }
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) o[n][m][j] += c[n][j];
             }
-        }
+        };
+        if (near) add_values(std::true_type{});
+        else add_values(std::false_type{});
         __syncwarp();   // buffer s is read
         if (it + NBUF < part_steps) issue(part, it + NBUF);
     }
 
-    // the warp's state to shared memory, O without the V factors' 2^(e - 24)
-    const float unscale = __uint_as_float((uint32_t)(127 + 24 - dexp) << 23);
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) o[n][m][k] *= unscale;
+    // the warp's state to shared memory
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll

@@ -64,3 +64,61 @@ def test_long_chunks_of_equal_tokens(heads, hd, kv, rows, past):
     worst = np.abs(out / v[None, :, None] - 1).max()
     assert worst <= 128 / 2 * 5 * 2.0 ** -23 + 64 * 2.0 ** -24 + 2.0 ** -22 + 17 * 2.0 ** -24, worst
     assert status() == 0
+
+
+def check_sizes(case, q, out, heads, seqs, ctx):
+    """As check_rows, relative to what each output sums instead of the largest value of all:
+    tolerance's factor times sum p |v|, and what a weight held as an fp16 pair may be off at
+    the bottom (2^-32 of the largest weight, for every token)."""
+    scale = 1 / np.sqrt(case.hd)
+    for r, (s, n) in enumerate(zip(seqs, ctx)):
+        for h in range(heads):
+            k, v = case.held(s, n, h // (heads // case.kv))
+            qh = q[r].reshape(heads, -1)[h].astype(np.float64)
+            p = np.exp((k @ qh) * scale - ((k @ qh) * scale).max())
+            p /= p.sum()
+            tol = km.tolerance(qh, k, np.ones((1, 1)), scale) * (p @ np.abs(v)) + 2.0 ** -32 * p.max() * np.abs(v).sum(0)
+            err = np.abs(out[r].reshape(heads, -1)[h] - p @ v)
+            assert (err <= tol).all(), (r, h, n, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("hd,heads,kv", [(32, 8, 2), (64, 14, 2), (128, 8, 2), (128, 4, 4), (128, 16, 1)])
+def test_values_of_very_different_size(hd, heads, kv):
+    """Blocks of dims and tokens whose values differ by up to 2^22, small ones with the weight."""
+    rng = np.random.default_rng(hd + heads)
+    n = 230
+    case = Case(rng, kv, hd, (n, n, n))
+    for b in range(hd // 32):                                   # sequence 0: by block of dims
+        case.v[0][..., 32 * b:32 * b + 32] *= 1000.0 * 10.0 ** (-2 * b)
+    case.v[1] *= np.exp2(rng.integers(-9, 13, (n, 1, 1))).astype(np.float32)     # 1: by token
+    u = rng.normal(0, 1, hd)                                    # 2: huge values of no weight
+    far = rng.permutation(n)[:n // 3]
+    case.v[2][far] *= 8000.0
+    for s in (1, 2):
+        case.v[s] = np.clip(case.v[s], -32768, 32768)
+    case.k[2][far] = (-60 * np.sqrt(hd) / (u @ u) * u).astype(np.float32)
+    case.k[2][[i for i in range(n) if i not in far]] *= 0.1
+    case.append(0, None)
+    q = rng.normal(0, 1, (3, heads * hd)).astype(np.float32)
+    q[2] = np.tile(u, heads)
+    out = case.cache.decode_attention(dev(q), heads, ints([n - 1] * 3)).cpu().numpy()
+    check_sizes(case, q, out, heads, range(3), [n] * 3)
+    out = run_chunks(case, np.repeat(q, 2, 0), heads, (2, 2, 2), (n - 2,) * 3).cpu().numpy()
+    check_sizes(case, np.repeat(q, 2, 0), out, heads, [0, 0, 1, 1, 2, 2], [n - 1, n] * 3)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("hd,heads,kv", [(64, 8, 2), (128, 8, 4), (128, 32, 8)])
+def test_later_rows_of_a_chunk_do_not_show_in_earlier_ones(hd, heads, kv):
+    """Draft rows whose last tokens hold the largest values there are: the rows before see none
+    of them, and come out as they do without them."""
+    rng = np.random.default_rng(hd * heads)
+    rows, past = 6, 87
+    case = Case(rng, kv, hd, (past + rows,))
+    q = rng.normal(0, 1, (rows, heads * hd)).astype(np.float32)
+    case.k[0][past + 3:] = 30000.0 * np.sign(rng.normal(0, 1, (3, kv, hd)))
+    case.v[0][past + 3:] = 30000.0
+    case.append(past, None)
+    out = run_chunks(case, q, heads, (rows,), (past,)).cpu().numpy()
+    check_rows(case, q[:3], out[:3], heads, [0] * 3, [past + 1, past + 2, past + 3])
+    check_sizes(case, q[:3], out[:3], heads, [0] * 3, [past + 1, past + 2, past + 3])
