@@ -13,12 +13,11 @@
 //   V: a nibble in place times D plus Z is (q - z) d 2^(e - 24) in one fused
 //      multiply-add, with D = d 2^e (high nibbles: d 2^(e - 4)) and Z = -z d
 //      2^(e - 24): exact while D is 2^6 to 2^16.  e is kept from step to step and
-//      moves when a step's d leave that window; where they are too far apart for any
+//      moves when a step's d leave that window.  Where they are too far apart for one
 //      (a factor of 2^9: tokens or blocks of dims of very different size, or a draft
-//      row's token that the others do not see), the step forms (q - z) d by a subtraction and
-//      a product, exact for every d, at a third instruction for a pair.  O is
-//      the plain sum either way.  (One e for all tokens so far, small d rounded,
-//      measured 0.5 us less of 54 at batch 64; the second form throughout, 3.2 more.)
+//      row's token that the others do not see), the smaller ones' (q - z) d are formed by
+//      a subtraction and a product, exact for every d, in a pass of their own.  O is the
+//      plain sum.  (With one e for all tokens so far, small d lost bits.)
 // Q (scaled by a power of two to below 2^14) and P (2^7 times the softmax
 // weight) are an fp16 high part plus an fp16 residual: results keep fp32
 // accuracy.  Up to four columns, the two parts are two columns of one product
@@ -291,6 +290,10 @@ struct NarrowCfg {
     static constexpr size_t SMEM = BAR + kNarrowWarps * NBUF * 8;
     static constexpr int JOIN_ITEMS = COLS * HD / 4 < 64 ? COLS * HD / 4 : 64;   // 4 dims of a column each
     static constexpr int CTAS = COLS <= 8 ? 3 : 2;   // resident per SM
+    // d below a step's window in a pass after the others', so that no branch stands before
+    // the products (64 x 2176 tokens of 32/4 heads of 64: 27.2 us, else 28.7); where 168
+    // registers do not hold that, all of the step's d instead (64/8 heads of 128: 39.3, else 40.7)
+    static constexpr bool AFTER = !(HD == 128 && COLS == 8);
 };
 
 // The parts of the tile that begins in run blockIdx.x, joined in page order: the
@@ -564,8 +567,10 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
     low = __reduce_min_sync(0xffffffffu, low);
 
     const float rest = t < 2 ? 0.0f : -1.0f;
-    int dexp = 0;                   // e, and the words of a step's scales that it takes:
-    uint32_t dlow = 0, dspan = 0;   // dlow .. dlow + dspan - 1
+    // e, and the scale words that it takes: dlow .. dlow + dspan - 1.  At first d of 2^-8 to
+    // 2^2, where the steps of values around 1 lie.
+    int dexp = 14;
+    uint32_t dlow = 7u << 10, dspan = 10u << 10;
     float o[NT][MT][4], base[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -592,56 +597,69 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
             tok0[p] = (bad >> (PP * s + p)) & 1 ? 0x40000000
                                                 : (part_b0 + (it * W + warp) * PP + p) * kKv4Tokens;
         // V factors: lane (g, t) makes those of block b = g % NB, tokens 2t + 8u, 2t + 1 + 8u
-        uint32_t dz[PP];
-        bool out = false;
-#pragma unroll
-        for (int p = 0; p < PP; p++) {
-            const uint8_t* vs = buf + p * F::BYTES + F::VS;
-            const int u = g / NB, r = 2 * t + 8 * (u & 1), b = g % NB;
-            uint32_t wa = *reinterpret_cast<const uint16_t*>(vs + F::scale(r, b));
-            uint32_t wb = *reinterpret_cast<const uint16_t*>(vs + F::scale(r + 1, b));
-            if (tok0[p] + kKv4Tokens > ctx) {   // slots behind the last token: any bits
-                if (tok0[p] + r >= ctx) wa = 0;
-                if (tok0[p] + r + 1 >= ctx) wb = 0;
-            }
-            out |= wa - dlow >= dspan || wb - dlow >= dspan;
-            dz[p] = __byte_perm(wa, wb, 0x5410);
-        }
-        bool near = true;
-        if (__any_sync(0xffffffffu, out)) {
-            uint32_t top = 0, low = 0xffffffffu;   // the largest and the smallest d, zeros aside, and some zero point
+        uint32_t wa[PP], wb[PP];
+        auto scale_words = [&](uint32_t hidden) {
 #pragma unroll
             for (int p = 0; p < PP; p++) {
-                top = max(top, max(dz[p] & 0xffffu, dz[p] >> 16));
-                low = min(low, min((dz[p] & 0xffffu) - 16u, (dz[p] >> 16) - 16u));
+                const uint8_t* vs = buf + p * F::BYTES + F::VS;
+                const int u = g / NB, r = 2 * t + 8 * (u & 1), b = g % NB;
+                wa[p] = *reinterpret_cast<const uint16_t*>(vs + F::scale(r, b));
+                wb[p] = *reinterpret_cast<const uint16_t*>(vs + F::scale(r + 1, b));
+                if (tok0[p] + kKv4Tokens > ctx) {   // slots behind the last token, any bits: their weights are 0
+                    if (tok0[p] + r >= ctx) wa[p] = hidden;
+                    if (tok0[p] + r + 1 >= ctx) wb[p] = hidden;
+                }
             }
-            top = __reduce_max_sync(0xffffffffu, top) >> 10;
-            low = __reduce_min_sync(0xffffffffu, low) + 16u;
-            if (low >> 10 == 0 && low >= 16) near = top <= 4;   // below 2^-14: down to 2^-20
-            else near = low < 16 || top <= (low >> 10) + 9;
-            if (near) {
-                const uint32_t spare = top <= 4 ? 0 : 9 - min(9u, low < 16 ? 0 : top - (low >> 10));
-                dexp = 30 - (int)(top + spare / 2);
-                dlow = dexp >= 26 ? 16 : (uint32_t)max(1, 21 - dexp) << 10;
-                dspan = ((uint32_t)(31 - dexp) << 10) - dlow;
-            }
-        }
-        if (near) {
+        };
+        auto put_factors = [&] {
             const uint32_t up1 = f16_pow2(dexp / 2), up2 = f16_pow2(dexp - dexp / 2);
 #pragma unroll
             for (int p = 0; p < PP; p++) {
-                const uint32_t D = hmul2u(hmul2u(dz[p] & 0x7ff07ff0u, up1), up2);
+                const uint32_t w = __byte_perm(wa[p], wb[p], 0x5410);
+                const uint32_t D = hmul2u(hmul2u(w & 0x7ff07ff0u, up1), up2);
                 if (g < 2 * NB)
                     *reinterpret_cast<uint2*>(vsc + p * C::VSC_PAGE + ((t * NB + g % NB) * 2 + g / NB) * 8) =
-                        make_uint2(D, hmul2u(dz[p] & 0x000f000fu, D) ^ 0x80008000u);
+                        make_uint2(D, hmul2u(w & 0x000f000fu, D) ^ 0x80008000u);
             }
-        } else {
+        };
+        auto put_far_factors = [&](uint32_t limit) {   // d below it
 #pragma unroll
-            for (int p = 0; p < PP; p++)
+            for (int p = 0; p < PP; p++) {
+                const uint32_t w = __byte_perm(wa[p] < limit ? wa[p] : 0, wb[p] < limit ? wb[p] : 0, 0x5410);
                 if (g < 2 * NB)
                     *reinterpret_cast<uint2*>(vsc + p * C::VSC_PAGE + ((t * NB + g % NB) * 2 + g / NB) * 8) =
-                        make_uint2(dz[p] & 0x7ff07ff0u, (dz[p] & 0x000f000fu) | 0x64006400u);
+                        make_uint2(w & 0x7ff07ff0u, (w & 0x000f000fu) | 0x64006400u);
+            }
+        };
+        scale_words(dlow);
+        bool out = false, left = false;
+#pragma unroll
+        for (int p = 0; p < PP; p++) out |= wa[p] - dlow >= dspan || wb[p] - dlow >= dspan;
+        if (__builtin_expect(__any_sync(0xffffffffu, out), 0)) {
+            // a window for the largest d, and for all the smaller ones if there is one
+            uint32_t top = 0, low = 0xffffffffu;
+#pragma unroll
+            for (int p = 0; p < PP; p++) {
+                top = max(top, max(wa[p], wb[p]));
+                low = min(low, min(wa[p] - 16u, wb[p] - 16u));   // zeros aside
+            }
+            top = __reduce_max_sync(0xffffffffu, top) >> 10;
+            low = __reduce_min_sync(0xffffffffu, low) + 16u;
+            low = low < 16 ? top : low >> 10;   // binades, 0 below 2^-14
+            const uint32_t spare = low == 0 || top > low + 9 ? 0 : (9 - (top - low)) / 2;
+            dexp = 30 - (int)(top + spare);
+            dlow = dexp >= 26 ? 16 : (uint32_t)max(1, 21 - dexp) << 10;
+            dspan = ((uint32_t)(31 - dexp) << 10) - dlow;
+#pragma unroll
+            for (int p = 0; p < PP; p++) {
+                left |= (wa[p] < dlow && wa[p] >= 16) || (wb[p] < dlow && wb[p] >= 16);
+                if (C::AFTER && wa[p] < dlow) wa[p] = 0;
+                if (C::AFTER && wb[p] < dlow) wb[p] = 0;
+            }
+            left = __any_sync(0xffffffffu, left);
         }
+        if (C::AFTER || !left) put_factors();
+        else put_far_factors(0x10000u);
         // scores: tokens g (sc[..][0], [1]) and g + 8 ([2], [3]), columns tq, tq + 1
         float sc[PP][NT][4];
 #pragma unroll
@@ -766,9 +784,9 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
         // largest term, so a step's products are summed from zero and added in
         // fp32: the error does not grow with the number of pages.
         constexpr int TPG = F::TPG;
-        const float back = __uint_as_float((uint32_t)(127 + 24 - dexp) << 23);
-        auto add_values = [&](auto is_near) {
-            constexpr bool NEAR = decltype(is_near)::value;
+        auto add_values = [&](auto by_window) {
+            constexpr bool WINDOW = decltype(by_window)::value;
+            const float back = __uint_as_float((uint32_t)(127 + 24 - dexp) << 23);
             // factors of tokens (2t, 2t + 1), (2t + 8, 2t + 9), and what high nibbles take instead
             uint32_t f2[PP][4], fh[PP][2];
 #pragma unroll
@@ -787,14 +805,14 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
                             lds_words<4>(f2[p], vsc + p * C::VSC_PAGE + (t * NB + b) * 16);
 #pragma unroll
                             for (int u = 0; u < 2; u++)   // D / 16, or 64 + z
-                                fh[p][u] = NEAR ? hmul2u(f2[p][2 * u], 0x2c002c00u)
-                                                : (f2[p][2 * u + 1] & 0x000f000fu) * 16 + 0x54005400u;
+                                fh[p][u] = WINDOW ? hmul2u(f2[p][2 * u], 0x2c002c00u)
+                                                  : (f2[p][2 * u + 1] & 0x000f000fu) * 16 + 0x54005400u;
                         }
                         uint32_t v[4];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             const uint32_t y = u ? x[p][k] >> 8 : x[p][k], d = f2[p][2 * u], z = f2[p][2 * u + 1];
-                            if constexpr (NEAR) {
+                            if constexpr (WINDOW) {
                                 v[2 * u] = hfma2u(y & 0x000f000fu, d, z);
                                 v[2 * u + 1] = hfma2u(y & 0x00f000f0u, fh[p][u], z);
                             } else {
@@ -812,12 +830,20 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) o[n][m][j] = fmaf(c[n][j], NEAR ? back : 1.0f, o[n][m][j]);
+                        for (int j = 0; j < 4; j++) o[n][m][j] = fmaf(c[n][j], WINDOW ? back : 1.0f, o[n][m][j]);
                 }
             }
         };
-        if (near) add_values(std::true_type{});
-        else add_values(std::false_type{});
+        if (C::AFTER || !left) add_values(std::true_type{});
+        if (__builtin_expect(left, 0)) {
+            if (C::AFTER) {
+                scale_words(0);
+                __syncwarp();   // the factors are read
+                put_far_factors(dlow);
+                __syncwarp();
+            }
+            add_values(std::false_type{});
+        }
         __syncwarp();   // buffer s is read
         if (it + NBUF < part_steps) issue(part, it + NBUF);
     }
