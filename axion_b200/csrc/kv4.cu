@@ -273,7 +273,7 @@ cudaError_t launch_narrow_cols(DeviceState* ds, const NarrowArgs& a, int ctas, c
     auto kern = kv4_attn_narrow_kernel<HD, COLS>;
     static std::atomic<int> configured[64] = {};   // by device
     const int dev = ds->device < 64 ? ds->device : 63;
-    if (smem > 48 * 1024 && (dev == 63 || !configured[dev])) {
+    if (dev == 63 || !configured[dev]) {   // with the kernel's static part, from less than 48 KB
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
         configured[dev] = 1;

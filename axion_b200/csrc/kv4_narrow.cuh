@@ -64,6 +64,11 @@ constexpr int kNarrowMinUnits = 14;   // units of a run at least elsewhere
 constexpr int kNarrowMaxParts = 96;   // parts of a tile at most (one CTA joins them)
 constexpr int kJoinThreads = 256;
 constexpr int kNarrowTileCost = 16;   // what a tile costs beside its pages, in pages
+// Pages of a part at most.  Weights and values that are alike round the same way at every
+// addition, so a CTA takes longer stretches of a tile in pieces and joins their states:
+// 64 sequences of 131072 equal tokens were 3.9e-5 off in one piece, 7.4e-6 now.  (Pieces
+// within a part, kept in shared memory by a rare branch of the loop, cost 3 % at any length.)
+constexpr int kNarrowPiece = 1024;
 constexpr int kNarrowKept = 128;      // entries kept in shared memory (else read again)
 
 struct Kv4Pages {
@@ -210,6 +215,7 @@ struct NarrowPart {
     int r0, cols, seq, pos0, ctx;   // the entry's first row, columns, sequence, first position, tokens
     int kvh, col0;                  // the tile
     int b0, b1;                     // pages of the part
+    int follows, ends;              // the CTA had the pages before in a part of its own; has none behind
     int c0, c1;                     // CTAs with parts of the tile; b0 == b1: no part
 };
 
@@ -250,12 +256,15 @@ __device__ __noinline__ void narrow_next_part(const NarrowArgs& a, const NarrowE
             d.kvh = seg % a.c.n_kv;
             d.col0 = seg / a.c.n_kv * COLS;
             d.b0 = max(0, p - tile);
-            d.b1 = last - tile;
+            d.b1 = min(last - tile, d.b0 + kNarrowPiece);
+            d.follows = d.b0 > 0 && p > (int)blockIdx.x * r.run;
+            d.ends = d.b1 == last - tile;
             d.c0 = tile / r.run;
             d.c1 = (tile + e.nblk - 1) / r.run;
+            p = d.ends ? stop : tile + d.b1;
+            break;
         }
         p = stop;
-        if (d.b1 > 0) break;
     }
     r.p = p;
     r.first = first;
@@ -287,7 +296,9 @@ struct NarrowCfg {
     static constexpr size_t QBUF = VSC + kNarrowWarps * PP * VSC_PAGE;   // Q of this and the next part
     static constexpr size_t KEPT = QBUF + 2 * COLS * HD * 4;
     static constexpr size_t BAR = KEPT + kNarrowKept * sizeof(NarrowEntry);
-    static constexpr size_t SMEM = BAR + kNarrowWarps * NBUF * 8;
+    static constexpr size_t PIECE = BAR + kNarrowWarps * NBUF * 8;   // of the pieces so far, in turn
+    static constexpr size_t PARTS = PIECE + 2 * COLS * 8;
+    static constexpr size_t SMEM = PARTS + 3 * sizeof(NarrowPart);
     static constexpr int JOIN_ITEMS = COLS * HD / 4 < 64 ? COLS * HD / 4 : 64;   // 4 dims of a column each
     static constexpr int CTAS = COLS <= 8 ? 3 : 2;   // resident per SM
     // d below a step's window in a pass after the others', so that no branch stands before
@@ -350,6 +361,75 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_attn_join_kernel(const __gri
     }
 }
 
+// The warps' states of a part, joined: out, or to the workspace where the tile has more.
+// A piece of a longer stretch joins those before it, whose sum rests in the same place (a
+// thread reads what itself wrote) and whose references and sums take turns in shared
+// memory.
+template <int HD, int COLS>
+__device__ __forceinline__ void narrow_merge(const NarrowArgs& a, int which, int turn) {
+    using C = NarrowCfg<HD, COLS>;
+    constexpr int W = kNarrowWarps;
+    extern __shared__ __align__(16) uint8_t nar_sm[];
+    const NarrowPart part = reinterpret_cast<const NarrowPart*>(nar_sm + C::PARTS)[which];
+    const float* acc_s = reinterpret_cast<const float*>(nar_sm + C::MERGE);
+    const float* ml_s = acc_s + (size_t)W * COLS * C::PITCH;
+    const float2* had = reinterpret_cast<const float2*>(nar_sm + C::PIECE) + turn * COLS;
+    float2* has = reinterpret_cast<float2*>(nar_sm + C::PIECE) + (turn ^ 1) * COLS;
+    const int c0 = part.c0, c1 = part.c1, live = min(COLS, part.cols - part.col0);
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (c0 == (int)blockIdx.x);
+    const bool out = c1 == c0 && part.ends;
+    for (int idx = threadIdx.x; idx < live * (HD / 4); idx += W * 32) {
+        const int col = idx / (HD / 4), d = idx % (HD / 4) * 4;
+        float mx = -CUDART_INF_F;
+#pragma unroll
+        for (int w = 0; w < W; w++) mx = fmaxf(mx, ml_s[(w * COLS + col) * 2]);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float mw = ml_s[(w * COLS + col) * 2];
+            const float f = mw == -CUDART_INF_F ? 0.0f : ex2(mw - mx);
+            const float4 x = *reinterpret_cast<const float4*>(acc_s + ((size_t)w * COLS + col) * C::PITCH + d);
+            v.x = fmaf(x.x, f, v.x);
+            v.y = fmaf(x.y, f, v.y);
+            v.z = fmaf(x.z, f, v.z);
+            v.w = fmaf(x.w, f, v.w);
+            sum = fmaf(ml_s[(w * COLS + col) * 2 + 1], f, sum);
+        }
+        float* at = a.part + (slot * COLS + col) * HD + d;
+        if (part.follows) {
+            const float2 ml = had[col];
+            if (ml.x != -CUDART_INF_F || ml.y != 0.0f) {   // else they saw nothing
+                const float4 was = *reinterpret_cast<const float4*>(at);
+                const float m = fmaxf(mx, ml.x), f = ex2(mx - m), h = ex2(ml.x - m);
+                v = make_float4(fmaf(v.x, f, was.x * h), fmaf(v.y, f, was.y * h), fmaf(v.z, f, was.z * h),
+                                fmaf(v.w, f, was.w * h));
+                sum = fmaf(sum, f, ml.y * h);
+                mx = m;
+            }
+        }
+        if (!out) {
+            *reinterpret_cast<float4*>(at) = v;
+            if (d == 0) {
+                has[col] = make_float2(mx, sum);
+                *reinterpret_cast<float2*>(a.part + (int64_t)gridDim.x * 2 * COLS * HD + (slot * COLS + col) * 2) =
+                    make_float2(mx, sum);
+            }
+        } else {
+            narrow_write(a, part, HD, col, d, v, sum);
+        }
+    }
+    if (c1 > c0 && c0 == (int)blockIdx.x && threadIdx.x == 0) a.split[blockIdx.x] = part;
+}
+
+// A function of its own leaves the page loop of 4 columns its registers: 131072 tokens
+// 51.0 us inlined, 50.5 called.  With 8 and 16 columns it is the other way: 32 x 2176 tokens
+// of 64/8 heads 39.2 and 39.8 us, 24 x 5 draft rows 35.9 and 36.9.
+template <int HD, int COLS>
+__device__ __noinline__ void narrow_merge_call(const NarrowArgs& a, int which, int turn) {
+    narrow_merge<HD, COLS>(a, which, turn);
+}
+
 template <int HD, int COLS>
 __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
     kv4_attn_narrow_kernel(const __grid_constant__ NarrowArgs a) {
@@ -381,7 +461,7 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
     NarrowEntry* kept = a.n_entries <= kNarrowKept ? reinterpret_cast<NarrowEntry*>(nar_sm + C::KEPT) : nullptr;
     __shared__ int scan_sm[2][2][W];
     __shared__ NarrowRun run_s;
-    __shared__ NarrowPart parts[3];     // the last, this and the next one
+    NarrowPart* parts = reinterpret_cast<NarrowPart*>(nar_sm + C::PARTS);   // the last, this and the next one
     {
         const int per = (a.n_entries + W * 32 - 1) / (W * 32), i0 = threadIdx.x * per;
         const int before = a.aligned ? 0 : kNarrowTileCost;
@@ -494,6 +574,7 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
     cp_async_wait_all();
     __syncthreads();   // Q is there, and the second part
 
+  int turn = 0;
   for (int which = 0, qb = 0;; which = which == 2 ? 0 : which + 1, qb ^= 1) {
     const NarrowPart& part = parts[which];
     const NarrowPart& next = parts[which == 2 ? 0 : which + 1];
@@ -781,8 +862,7 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
             }
         }
         // O^T += V^T P^T.  A product truncates what it adds to about 24 bits of the
-        // largest term, so a step's products are summed from zero and added in
-        // fp32: the error does not grow with the number of pages.
+        // largest term, so a step's products are summed from zero and added in fp32.
         constexpr int TPG = F::TPG;
         auto add_values = [&](auto by_window) {
             constexpr bool WINDOW = decltype(by_window)::value;
@@ -892,36 +972,9 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
     }
     cp_async_wait_all();
     __syncthreads();   // states, and the next part's Q
-    const int c0 = part.c0, c1 = part.c1, live = min(COLS, part.cols - part.col0);
-    const int64_t slot = (int64_t)blockIdx.x * 2 + (c0 == (int)blockIdx.x);
-    for (int idx = threadIdx.x; idx < live * (HD / 4); idx += W * 32) {
-        const int col = idx / (HD / 4), d = idx % (HD / 4) * 4;
-        float mx = -CUDART_INF_F;
-#pragma unroll
-        for (int w = 0; w < W; w++) mx = fmaxf(mx, ml_s[(w * COLS + col) * 2]);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float mw = ml_s[(w * COLS + col) * 2];
-            const float f = mw == -CUDART_INF_F ? 0.0f : ex2(mw - mx);
-            const float4 x = *reinterpret_cast<const float4*>(acc_s + ((size_t)w * COLS + col) * C::PITCH + d);
-            v.x = fmaf(x.x, f, v.x);
-            v.y = fmaf(x.y, f, v.y);
-            v.z = fmaf(x.z, f, v.z);
-            v.w = fmaf(x.w, f, v.w);
-            sum = fmaf(ml_s[(w * COLS + col) * 2 + 1], f, sum);
-        }
-        if (c1 > c0) {
-            *reinterpret_cast<float4*>(a.part + (slot * COLS + col) * HD + d) = v;
-            if (d == 0)
-                *reinterpret_cast<float2*>(a.part + (int64_t)gridDim.x * 2 * COLS * HD + (slot * COLS + col) * 2) =
-                    make_float2(mx, sum);
-        } else {
-            narrow_write(a, part, HD, col, d, v, sum);
-        }
-    }
-    if (c1 > c0 && c0 == (int)blockIdx.x && threadIdx.x == 0) a.split[blockIdx.x] = part;
+    if constexpr (COLS <= 4) narrow_merge_call<HD, COLS>(a, which, turn);
+    else narrow_merge<HD, COLS>(a, which, turn);
+    turn ^= 1;
     if (!more) break;
   }
 }

@@ -66,6 +66,37 @@ def test_long_chunks_of_equal_tokens(heads, hd, kv, rows, past):
     assert status() == 0
 
 
+def test_many_long_sequences_of_equal_tokens():
+    """64 sequences over the same 131,072 tokens, each page a copy of the first: a CTA walks
+    thousands of pages of one tile.  It takes 1024 of them at a time, 256 a warp: 256 additions
+    of weights, and of products, of at most 2^-24 of sums that grow evenly; a step's products
+    start from zero, 4 instructions of at most 5 units of 2^-23 (test_long_chunks_of_equal_tokens);
+    2^-22 for the weights' pairs; 8 pieces and 4 warps of 2^-24.  (3.9e-5 off in one chain.)"""
+    limit = 2 * 256 / 2 * 2.0 ** -24 + 4 * 5 * 2.0 ** -23 + 2.0 ** -22 + 12 * 2.0 ** -24
+    from axion_b200.paged_kv import PagedKVCache4
+    rng = np.random.default_rng(64)
+    n, kv, hd, heads = 131072, 8, 128, 32
+    k, v = rng.normal(0, 1, (kv, hd)).astype(np.float32), rng.uniform(0.5, 1.5, (kv, hd)).astype(np.float32)
+    pages = torch.empty(n // 16, kv, 18 * hd, dtype=torch.uint8, device="cuda")
+    table = np.tile(np.arange(n // 16, dtype=np.int32), (64, 1))
+    cache = PagedKVCache4(kv, hd, pages=pages, block_table=dev(table))
+    kd, vd = (dev(x.reshape(1, -1)).repeat(16, 1) for x in (k, v))
+    kd[3] *= 1.25                               # not every weight is a power of two
+    cache.append_rows(kd, vd, ints([0] * 16), ints(range(16)))
+    pages[1:] = pages[0]
+    held = km.values(v)
+    for per, seqs in ((1, 64), (4, 48)):       # 4 columns of a tile, and 16
+        q = rng.normal(0, 1, (seqs * per, heads * hd)).astype(np.float32)
+        if per == 1:
+            out = cache.decode_attention(dev(q), heads, ints([n - 1] * seqs))
+        else:
+            out = cache.chunk_attention(dev(q), heads, ints(range(0, seqs * per + 1, per)), ints([n - per] * seqs), per)
+        out = out.cpu().numpy().reshape(seqs * per, kv, -1, hd)
+        worst = np.abs(out / held[None, :, None] - 1).max()
+        assert worst <= limit, (per, worst)
+    assert status() == 0
+
+
 def check_sizes(case, q, out, heads, seqs, ctx):
     """As check_rows, relative to what each output sums instead of the largest value of all:
     tolerance's factor times sum p |v|, and what a weight held as an fp16 pair may be off at
@@ -122,3 +153,34 @@ def test_later_rows_of_a_chunk_do_not_show_in_earlier_ones(hd, heads, kv):
     out = run_chunks(case, q, heads, (rows,), (past,)).cpu().numpy()
     check_rows(case, q[:3], out[:3], heads, [0] * 3, [past + 1, past + 2, past + 3])
     check_sizes(case, q[:3], out[:3], heads, [0] * 3, [past + 1, past + 2, past + 3])
+
+
+@pytest.mark.parametrize("heads,hd,kv,rows", [(8, 128, 2, 1), (14, 64, 2, 1), (16, 32, 1, 1), (8, 128, 2, 5)])
+def test_every_page_of_a_long_context_counts(heads, hd, kv, rows):
+    """20,011 tokens in a split context, 1e-5 of the result's norm: a page lost or taken twice at a
+    seam is about 8e-4 of the weight, 80 times that.  The bound: scores 16 products each dropping
+    at most 2^-23 of a sum |q k| / sqrt(hd) of about 2, 4e-6; weights 2^-22; sums in pieces of
+    at most 32 additions of 2^-24, 2e-6."""
+    rng = np.random.default_rng(heads + rows)
+    n = 20011
+    case = Case(rng, kv, hd, (n, n - 777))
+    for s in range(2):
+        case.v[s][:] = np.abs(case.v[s]) + 0.5
+    case.append(0, None)
+    q = rng.normal(0, 0.3, (2 * rows, heads * hd)).astype(np.float32)
+    if rows == 1:
+        out = case.cache.decode_attention(dev(q), heads, ints(x - 1 for x in case.lens))
+    else:
+        out = run_chunks(case, q, heads, (rows, rows), [x - rows for x in case.lens])
+    out = out.cpu().numpy().reshape(2 * rows, heads, hd)
+    for s in range(2):
+        for kvh in range(kv):
+            k, v = case.held(s, case.lens[s], kvh)
+            for r in {0, rows - 1}:
+                m = case.lens[s] - rows + r + 1
+                for h in range(kvh * heads // kv, (kvh + 1) * heads // kv, 3):
+                    qh = q[s * rows + r].reshape(heads, hd)[h].astype(np.float64)
+                    ref = km.attention(qh, k[:m], v[:m], 1 / np.sqrt(hd))
+                    err = np.linalg.norm(out[s * rows + r, h] - ref) / np.linalg.norm(ref)
+                    assert err <= 1e-5, (s, r, h, err)
+    assert status() == 0
