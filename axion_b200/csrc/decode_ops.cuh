@@ -224,11 +224,17 @@ inline size_t attn_smem_bytes(int G, int cp, int bps) {
            ((size_t)bps * sizeof(int) + 15) / 16 * 16;
 }
 
+// A page id as the pools take it: one outside them (a table entry without a page) reads
+// their last page, so that nothing is read beyond.
+__device__ __forceinline__ int pool_page(int id, int n_pages) {
+    return (int)min((unsigned)id, (unsigned)n_pages - 1u);
+}
+
 template <typename KV, int HD, bool Q8>
 __global__ void attn_decode_kernel(const float* __restrict__ qkv, int ldq,
                                    const int* __restrict__ pos, const KV* __restrict__ kc,
                                    const KV* __restrict__ vc, const int* __restrict__ block_table,
-                                   int max_blocks, int n_heads, int n_kv, int bps, int cp,
+                                   int max_blocks, int n_pages, int n_heads, int n_kv, int bps, int cp,
                                    float scale, float* __restrict__ part, int* __restrict__ counters,
                                    float* __restrict__ out, int8_t* __restrict__ xq,
                                    float* __restrict__ dx, int dxt) {
@@ -249,7 +255,7 @@ __global__ void attn_decode_kernel(const float* __restrict__ qkv, int ldq,
     // the page table is written by the host before the step: read it while
     // the previous kernel drains
     for (int i = threadIdx.x; i < bps; i += blockDim.x)
-        pg[i] = b0 + i < max_blocks ? block_table[m * max_blocks + b0 + i] : 0;
+        pg[i] = b0 + i < max_blocks ? pool_page(block_table[m * max_blocks + b0 + i], n_pages) : 0;
     pdl_launch_dependents();
     pdl_wait();
     // a position past the page table was already reported by the KV append;
@@ -476,7 +482,7 @@ template <int HD, bool Q8>
 __global__ void __launch_bounds__(kAttnTcWarps * 32)
     attn_tc_kernel(const float* __restrict__ qkv, int ldq, const int* __restrict__ pos,
                    const __half* __restrict__ kc, const __half* __restrict__ vc,
-                   const int* __restrict__ block_table, int max_blocks, int n_heads, int n_kv,
+                   const int* __restrict__ block_table, int max_blocks, int n_pages, int n_heads, int n_kv,
                    int G, int bps, float scale, float* __restrict__ part, int* __restrict__ counters,
                    float* __restrict__ out, int8_t* __restrict__ xq, float* __restrict__ dx, int dxt) {
     constexpr int B = 16;
@@ -493,7 +499,7 @@ __global__ void __launch_bounds__(kAttnTcWarps * 32)
     const int g = lane >> 2, t = lane & 3;
     const int b0 = s * bps;
     for (int i = threadIdx.x; i < bps; i += blockDim.x)
-        pg[i] = b0 + i < max_blocks ? block_table[m * max_blocks + b0 + i] : 0;
+        pg[i] = b0 + i < max_blocks ? pool_page(block_table[m * max_blocks + b0 + i], n_pages) : 0;
     pdl_launch_dependents();
     pdl_wait();
     const int ctx = min(ld_cg(pos + m) + 1, max_blocks * B);
@@ -688,7 +694,7 @@ template <int HD, bool Q8>
 __global__ void __launch_bounds__(kAttnTcWarps * 32)
     attn_tct_kernel(const float* __restrict__ qkv, int ldq, const int* __restrict__ pos,
                     const __half* __restrict__ kc, const __half* __restrict__ vc,
-                    const int* __restrict__ block_table, int max_blocks, int n_heads, int n_kv,
+                    const int* __restrict__ block_table, int max_blocks, int n_pages, int n_heads, int n_kv,
                     int G, int bps, float scale, float* __restrict__ part, int* __restrict__ counters,
                     float* __restrict__ out, int8_t* __restrict__ xq, float* __restrict__ dx, int dxt) {
     constexpr int B = 16;
@@ -706,7 +712,7 @@ __global__ void __launch_bounds__(kAttnTcWarps * 32)
     const int g = lane >> 2, t = lane & 3;
     const int b0 = s * bps;
     for (int i = threadIdx.x; i < bps; i += blockDim.x)
-        pg[i] = b0 + i < max_blocks ? block_table[m * max_blocks + b0 + i] : 0;
+        pg[i] = b0 + i < max_blocks ? pool_page(block_table[m * max_blocks + b0 + i], n_pages) : 0;
     pdl_launch_dependents();
     pdl_wait();
     const int ctx = min(ld_cg(pos + m) + 1, max_blocks * B);
@@ -979,7 +985,7 @@ template <int HD, bool Q8>
 __global__ void __launch_bounds__(kPrefWarps * 32)
     attn_prefill_kernel(const float* __restrict__ qkv, int ldq, int T, int p0,
                         const __half* __restrict__ kc, const __half* __restrict__ vc,
-                        const int* __restrict__ block_table, int max_blocks, int n_kv, int G,
+                        const int* __restrict__ block_table, int max_blocks, int n_pages, int n_kv, int G,
                         float scale, int8_t* __restrict__ xq, int ldo, float* __restrict__ dxT,
                         int dxt, float* __restrict__ out) {
     constexpr int B = 16;
@@ -1014,7 +1020,7 @@ __global__ void __launch_bounds__(kPrefWarps * 32)
             const int j = c / (B * CH), r = (c / CH) % B, ch = c % CH;
             const int pg = st * SP + j;
             if (pg >= npages) continue;
-            const int64_t off = (((int64_t)bt[pg] * n_kv + kvh) * B + r) * HD + ch * 8;
+            const int64_t off = (((int64_t)pool_page(bt[pg], n_pages) * n_kv + kvh) * B + r) * HD + ch * 8;
             const int sw = r * HD + ((ch ^ (r & 7)) * 8);
             __half* kb = buf + (size_t)j * 2 * PAGE;
             cp_async16(kb + sw, kc + off);

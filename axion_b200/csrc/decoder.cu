@@ -81,7 +81,7 @@ struct axdec_model {
     bool out_set = false;
     float* out_norm = nullptr;
     std::vector<Layer> L;
-    int max_blocks = 0, nsplit = 1, bps = 1;
+    int max_blocks = 0, n_pages = 0, nsplit = 1, bps = 1;
     // activations
     float* h = nullptr;           // [M, H] residual stream
     int8_t* xq = nullptr;         // [M, maxK]
@@ -450,7 +450,7 @@ int launch_attention(axdec_model* m, int M, int layer, cudaStream_t s, int dxt) 
         AXQ8_CUDA_TRY(launch_k(kern, dim3(c.n_kv_heads, M, m->nsplit), dim3(kAttnTcWarps * 32),
                                smem, s, true, (const float*)m->qkv, m->Nqkv, (const int*)m->pos,
                                (const __half*)Ly.kc, (const __half*)Ly.vc,
-                               (const int*)m->block_table, m->max_blocks, c.n_heads,
+                               (const int*)m->block_table, m->max_blocks, m->n_pages, c.n_heads,
                                c.n_kv_heads, G, m->bps, scale, m->part, m->attn_cnt, m->x32,
                                m->xq, m->dx, dxt),
                       "attention launch");
@@ -468,7 +468,7 @@ int launch_attention(axdec_model* m, int M, int layer, cudaStream_t s, int dxt) 
     auto kern = q8 ? attn_decode_kernel<KV, HD, true> : attn_decode_kernel<KV, HD, false>;
     AXQ8_CUDA_TRY(launch_k(kern, dim3(c.n_kv_heads, M, m->nsplit), dim3(G * 32), smem, s, true,
                            (const float*)m->qkv, m->Nqkv, (const int*)m->pos, (const KV*)Ly.kc,
-                           (const KV*)Ly.vc, (const int*)m->block_table, m->max_blocks, c.n_heads,
+                           (const KV*)Ly.vc, (const int*)m->block_table, m->max_blocks, m->n_pages, c.n_heads,
                            c.n_kv_heads, m->bps, cp, scale, m->part, m->attn_cnt, m->x32, m->xq,
                            m->dx, dxt),
                   "attention launch");
@@ -890,7 +890,7 @@ int launch_attn_prefill(axdec_model* m, int layer, int n_seq, int T, int p0, int
     AXQ8_CUDA_TRY(launch_k(kern, dim3((unsigned)(((T + TQ - 1) / TQ) * HG), c.n_kv_heads, n_seq),
                            dim3(kPrefWarps * 32), smem, s, true, (const float*)m->pqkv, m->Nqkv, T,
                            p0, (const __half*)Ly.kc, (const __half*)Ly.vc,
-                           (const int*)m->block_table, m->max_blocks, c.n_kv_heads, G, scale,
+                           (const int*)m->block_table, m->max_blocks, m->n_pages, c.n_kv_heads, G, scale,
                            m->pxq, m->Nq, m->pdx, dxt, (float*)nullptr),
                   "prefill attention launch");
     return AXQ8_OK;
@@ -1141,6 +1141,7 @@ int axdec_create(const axdec_config_t* cfg, axdec_model_t** out) {
     const int M = c.max_batch, H = c.hidden, F = c.ffn;
     const size_t kvsz = c.kv_fp32 ? 4 : 2;
     const int64_t pages = (int64_t)M * m->max_blocks;
+    m->n_pages = (int)pages;
     m->embd = (uint8_t*)dalloc(m, (size_t)cf.vocab * m->rs_h, &rc);   // replicated
     m->out_w = (uint8_t*)dalloc(m, (size_t)c.vocab * m->rs_h, &rc);
     m->out_norm = (float*)dalloc(m, sizeof(float) * H, &rc);

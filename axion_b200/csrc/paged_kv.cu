@@ -94,7 +94,7 @@ int launch_attn(DeviceState* ds, const axkv_cache_t* c, const float* q, int n_se
             }
             AXQ8_CUDA_TRY(launch_k(kern, dim3(c->n_kv_heads, n_seq, nsplit), dim3(kAttnTcWarps * 32),
                                    smem, s, false, q, n_heads * HD, q_pos, (const __half*)c->k_pages,
-                                   (const __half*)c->v_pages, c->block_table, c->max_blocks, n_heads,
+                                   (const __half*)c->v_pages, c->block_table, c->max_blocks, c->n_pages, n_heads,
                                    c->n_kv_heads, G, bps, scale, part, counters, out,
                                    (int8_t*)nullptr, (float*)nullptr, 0),
                           "axkv_paged_decode_attn launch");
@@ -107,7 +107,7 @@ int launch_attn(DeviceState* ds, const axkv_cache_t* c, const float* q, int n_se
     AXQ8_CUDA_TRY(launch_k(attn_decode_kernel<KV, HD, false>, dim3(c->n_kv_heads, n_seq, nsplit),
                            dim3(G * 32), smem, s, false, q, n_heads * HD, q_pos,
                            (const KV*)c->k_pages, (const KV*)c->v_pages, c->block_table,
-                           c->max_blocks, n_heads, c->n_kv_heads, bps, cp, scale, part, counters,
+                           c->max_blocks, c->n_pages, n_heads, c->n_kv_heads, bps, cp, scale, part, counters,
                            out, (int8_t*)nullptr, (float*)nullptr, 0),
                   "axkv_paged_decode_attn launch");
     return AXQ8_OK;
@@ -128,7 +128,7 @@ int prefill_launch(DeviceState* ds, const axkv_cache_t* c, dim3 grid, const floa
     }
     AXQ8_CUDA_TRY(launch_k(kern, grid, dim3(kPrefWarps * 32), smem, s, false, q, (int)ldq, T, p0,
                            (const __half*)c->k_pages, (const __half*)c->v_pages, c->block_table,
-                           c->max_blocks, c->n_kv_heads, G, scale, xq, n_heads * HD, dxT, dxt, out),
+                           c->max_blocks, c->n_pages, c->n_kv_heads, G, scale, xq, n_heads * HD, dxT, dxt, out),
                   "axkv_paged_prefill_attn launch");
     return AXQ8_OK;
 }

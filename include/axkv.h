@@ -5,8 +5,11 @@
  * arrays of pages [n_pages][n_kv_heads][page_tokens][head_dim] (fp16, or fp32
  * with kv_fp32 = 1); token p of sequence s lives in page
  * block_table[s * max_blocks + p / page_tokens], slot p % page_tokens (the
- * block table is a caller-owned device array of int32).  Same conventions as
- * axq8.h: plain C, status codes, axq8_last_error().
+ * block table is a caller-owned device array of int32).  A page id outside the
+ * pool (-1: no page) is left out by an append, which reports it in the device
+ * status word; decode and prefill attention read the pool's last page in its
+ * place, so that row's result is undefined and nothing is read beyond.  Same
+ * conventions as axq8.h: plain C, status codes, axq8_last_error().
  *
  * Reference interfaces replaced (paths inside the reference project):
  *   PagedKVCache::initialize / append   inference/cpp/runtime/paged_kv.hpp:18-41,
