@@ -22,6 +22,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200, sm_100a)")
 
 
+def pytest_collection_modifyitems(items):
+    """The test of the C++ boundary goes last: its binary is built from the reference's sources,
+    and where they are absent it fails, behind which a run that stops at the first failure would
+    leave every other test out."""
+    items.sort(key=lambda item: item.name == "test_boundary_against_reference")
+
+
 @pytest.fixture(scope="session")
 def oracle():
     from oracle.oracle import Oracle
