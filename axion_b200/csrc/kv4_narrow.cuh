@@ -18,18 +18,20 @@
 //      row's token that the others do not see), the smaller ones' (q - z) d are formed by
 //      a subtraction and a product, exact for every d, in a pass of their own.  O is the
 //      plain sum.  (With one e for all tokens so far, small d lost bits.)
-// Q (scaled by a power of two to below 2^14) and P (2^7 times the softmax
-// weight) are an fp16 high part plus an fp16 residual: results keep fp32
-// accuracy.  Up to four columns, the two parts are two columns of one product
-// (no padding, half the products); beyond, two products into one accumulator.  Softmax in base 2 with a running reference;
-// it moves (and O is rescaled) only when a score exceeds it by more than 8, so
-// that weights stay within fp16.
+// Q (scaled by a power of two to below 2^11) is a whole number plus an fp16 residual:
+// whole numbers times codes sum without loss, so only the residual's products are cut
+// (with an fp16 high part instead, 257 tokens were 1.8e-6 off and 64 x 2176 9e-7; now
+// 5.5e-7 and 2.7e-7, and sums in fp32 5.8e-7 and 1.0e-6).  P (2^7 times the softmax
+// weight) is an fp16 high part plus an fp16 residual.  Up to four columns, the two parts
+// are two columns of one product (no padding, half the products); beyond, two products
+// into one accumulator.  Softmax in base 2 with a running reference; it moves (and O is
+// rescaled) only when a score exceeds it by more than 8, so that weights stay within fp16.
 //
-// The pages of all tiles (entry, column tile, KV head) in a row are dealt out
-// in equal runs to as many CTAs as the GPU holds at once, whatever the
-// sequences' lengths; a CTA walks the parts of tiles that its run covers (one
-// part where there are twice as many CTAs as tiles: every tile then starts a
-// run).  Its
+// The pages of all tiles (entry, column tile, KV head) in a row are dealt out in
+// equal runs to as many CTAs as the GPU holds at once, whatever the sequences'
+// lengths; a CTA walks the parts of tiles that its run covers.  Where there are at
+// least twice as many CTAs as tiles, a tile's length is rounded up to whole runs, so
+// that every tile starts one and a CTA has one part.  Its
 // kNarrowWarps warps take a part's pages in turn, two at a time where registers
 // allow (one softmax step and twice the independent products).  Each has its
 // own ring of page buffers, filled by bulk copies (a page's 18 HD bytes of one
@@ -38,8 +40,8 @@
 // tile through the workspace in a second kernel, in page order.
 //
 // Bound: issue slots.  64 sequences of 2176 tokens (32 query, 8 KV heads of 128):
-// 55 us, 162 MB, 0.47 of the measured copy bandwidth, about 415 instructions a
-// page at 0.59 of the slots; one sequence of 131072 tokens: 51 us.  Three CTAs an
+// 55 us, 162 MB, 0.46 of the measured copy bandwidth, about 414 instructions a
+// page at 0.59 of the slots; one sequence of 131072 tokens: 50 us.  Three CTAs an
 // SM measured 51 us there, four (fewer registers) 54; one page a step 56 against
 // 55 us at batch 64.
 #pragma once
@@ -61,7 +63,7 @@ constexpr int kNarrowWarps = 4;
 constexpr int kNarrowPages = 4;       // page buffers of a warp
 constexpr int kNarrowMinPages = 24;   // pages of a run at least, where every tile starts one
 constexpr int kNarrowMinUnits = 14;   // units of a run at least elsewhere
-constexpr int kNarrowMaxParts = 96;   // parts of a tile at most (one CTA joins them)
+constexpr int kNarrowMaxParts = 96;   // a run is at least that share of the longest tile: 97 parts at most
 constexpr int kJoinThreads = 256;
 constexpr int kNarrowTileCost = 16;   // what a tile costs beside its pages, in pages
 // Pages of a part at most.  Weights and values that are alike round the same way at every
@@ -307,7 +309,8 @@ struct NarrowCfg {
     static constexpr bool AFTER = !(HD == 128 && COLS == 8);
 };
 
-// The parts of the tile that begins in run blockIdx.x, joined in page order: the
+// The parts of the tile that begins in run blockIdx.x, joined in page order by one CTA
+// for every JOIN_ITEMS groups of 4 dims: the
 // second slot of CTA c0, then the first slots of c0 + 1 .. c1.  Groups of threads
 // take every S-th part of a column's 4 dims each; group states join the same way.
 template <int HD, int COLS>
@@ -601,10 +604,10 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
             }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // 2^k with max |q| 2^k in [2^13, 2^14)
+        // 2^k with max |q| 2^k in [2^10, 2^11)
         const int ex = max((int)(__float_as_uint(mx) >> 23), 40) - 127;
-        const float up = __uint_as_float((uint32_t)(127 + 13 - ex) << 23);
-        const float down = __uint_as_float((uint32_t)(127 - 13 + ex) << 23) * 16777216.0f * a.scale;
+        const float up = __uint_as_float((uint32_t)(127 + 10 - ex) << 23);
+        const float down = __uint_as_float((uint32_t)(127 - 10 + ex) << 23) * 16777216.0f * a.scale;
         float sum[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -614,8 +617,8 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
             for (int k = 0; k < 4; k++) {
                 const float f = k < 2 ? 1.0f : 0.0625f;
                 const float x0 = x[b][first[k]] * up, x1 = x[b][first[k] + 4] * up;
-                uint32_t hi, lo;
-                split2(x0 * f, x1 * f, hi, lo);
+                const float r0 = rintf(x0), r1 = rintf(x1);
+                const uint32_t hi = pack_f16(r0 * f, r1 * f), lo = pack_f16((x0 - r0) * f, (x1 - r1) * f);
                 if (PACK) {   // columns 4 .. 7 are the residuals of columns 0 .. 3
                     qh[n][b][k] = g < 4 ? hi : lo;
                     const float2 v = f16_pair(qh[n][b][k]);
@@ -771,9 +774,7 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
                     if constexpr (PACK) {
                         mma_f16_16816_first(c, lowa, qh[n][b][0], qh[n][b][1]);
                     } else {
-                        // residuals last: first, they cost half the accuracy (2.4e-6
-                        // against 1.1e-6 on the whole), as a product drops what is
-                        // far below its largest term
+                        // residuals last: the sum before them is exact
                         mma_f16_16816_first(c, lowa, qh[n][b][0], qh[n][b][1]);
                         mma_f16_16816(c, higha, qh[n][b][2], qh[n][b][3]);
                         mma_f16_16816(c, lowa, ql[n][b][0], ql[n][b][1]);
