@@ -373,9 +373,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
             const int sees = __reduce_min_sync(0xffffffffu, live ? pos : 0x7fffffff);
             const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * C::TILE_COLS, to = ts + 128;
             const int64_t oat = (int64_t)(r0 + j) * a.n_heads * HD + (int64_t)(kvh * a.G + min(m, rows - 1) - j * a.G) * HD;
-            // the weights' sum and what its additions lost (equal weights lose the same at each: a
-            // plain sum was 1.2e-4 off at 16,000 tokens), and the sum of a step
-            float base = -CUDART_INF_F, l = 0.0f, l_lost = 0.0f, l_step[2] = {0.0f, 0.0f};
+            // the weights' sum and what its additions put over (equal weights round the same way at
+            // each: a plain sum was 1.3e-4 off at 16,000 tokens), and the sum of a step
+            float base = -CUDART_INF_F, l = 0.0f, l_over = 0.0f, l_step[2] = {0.0f, 0.0f};
             float kept = -CUDART_INF_F;   // the reference of the sum in `out`
             uint32_t s[2][32];   // 32 tokens each, the next ones on their way
             for (int st = 0; st < steps; st++) {
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                         base = to_base;
                         const float f = __uint_as_float((uint32_t)(127 + down) << 23);
                         l *= f;
-                        l_lost *= f;
+                        l_over *= f;
                         l_step[0] *= f;
                         l_step[1] *= f;
                         // what is on its way has to arrive before its registers can be moved
@@ -430,8 +430,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                         for (int e = 0; e < 8; e++) {
                             const float w0 = ex2(fmaf(__uint_as_float(v[16 * p + 2 * e]), mul, -b7));
                             const float w1 = ex2(fmaf(__uint_as_float(v[16 * p + 2 * e + 1]), mul, -b7));
-                            l_step[0] += w0;
-                            l_step[1] += w1;
+                            l_step[0] = c || p || e ? l_step[0] + w0 : w0;
+                            l_step[1] = c || p || e ? l_step[1] + w1 : w1;
                             split2(w0, w1, hi[e], lo[e]);
                         }
                         tmem_st8(ts + 32 * c + 8 * p, hi);
@@ -441,17 +441,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv4_attn_wide_kernel(const __
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(pfull + x);
-                const float add = l_step[0] + l_step[1], sum = l + add, had = sum - add;
-                l_lost += (l - had) + (add - (sum - had));
+                const float add = l_step[0] + l_step[1] - l_over, sum = l + add;
+                l_over = (sum - l) - add;
                 l = sum;
-                l_step[0] = l_step[1] = 0.0f;
             }
             // O / l: the tile's rows to shared memory (Q and K are read), from there to `out`
             if (!lost) lost = !wide_wait(odone + x, 0, stop, a.status);
             __syncwarp();
             tc_fence_after();
             if (steps > kWideKeep) wide_keep<HD>(to, a.out, oat, live, true, true, wide_down(kept, base));
-            const float sum = l + l_lost;
+            const float sum = l - l_over;
             const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;   // nothing seen: zeros
             uint8_t* orow = sm + (128 * x + r) * C::OROW;
 #pragma unroll
