@@ -617,7 +617,8 @@ __global__ void __launch_bounds__(kNarrowWarps * 32, NarrowCfg<HD, COLS>::CTAS)
             for (int k = 0; k < 4; k++) {
                 const float f = k < 2 ? 1.0f : 0.0625f;
                 const float x0 = x[b][first[k]] * up, x1 = x[b][first[k] + 4] * up;
-                const float r0 = rintf(x0), r1 = rintf(x1);
+                // rounded to whole numbers by the addition
+                const float r0 = (x0 + 12582912.0f) - 12582912.0f, r1 = (x1 + 12582912.0f) - 12582912.0f;
                 const uint32_t hi = pack_f16(r0 * f, r1 * f), lo = pack_f16((x0 - r0) * f, (x1 - r1) * f);
                 if (PACK) {   // columns 4 .. 7 are the residuals of columns 0 .. 3
                     qh[n][b][k] = g < 4 ? hi : lo;
