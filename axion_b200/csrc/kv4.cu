@@ -350,8 +350,14 @@ cudaError_t launch_wide(DeviceState* ds, const axkv4_cache_t* c, const float* q,
 
 // Whether the tensor-core tiles of 256 rows (kv4_wide.cuh) take a chunk call, or the
 // column tiles of 16 (kv4_narrow.cuh), which share a long context among all SMs.
-// Measured per page of context: a CTA of the first takes 0.61 us, whatever its
-// rows, one to an SM; a tile of the second 0.27 us of an SM.
+// Measured per page of context at head dim 128 (64 and 32): a CTA of the first takes
+// 0.67 us (0.48, 0.44), whatever its rows, one to an SM, and no other SM helps it; a tile
+// of the second 0.18 us of an SM (0.12, 0.10), so the head dim hardly matters.  From a
+// prompt's start a tile of the second walks twice the pages it needs, and short contexts
+// cost it more beside the pages: 61 to 27 lies between the two.  18 chunks of 12 rows of
+// 32/8 heads: 349 us (the second 276) over 8192 tokens, 61 (62) over 1024, 14.5 (20.8)
+// from the start; 2 chunks of 64 rows over 8192 tokens 324 (171, taken), of 100 rows from
+// the start 16.5 (26.7).  Furthest off: 4 prompts of 40 rows take 22.6, 15.6 by the first.
 bool wide_takes(DeviceState* ds, const axkv4_cache_t* c, int chunks, int rows, int G) {
     const int64_t cols = (int64_t)rows * G, lists = (int64_t)chunks * c->n_kv_heads;
     const int64_t waves = (lists * ((cols + 255) / 256) + ds->sm_count - 1) / ds->sm_count;

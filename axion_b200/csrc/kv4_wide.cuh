@@ -10,8 +10,8 @@
 // shared memory without rounding (128-byte-swizzled K-major rows), once for
 // both tiles.  Q (scaled per row by a power of two to below 2^14) and P (2^7
 // times the softmax weight) are an fp16 high part plus an fp16 residual,
-// multiplied one after the other: results keep fp32 accuracy at twice the
-// products.  Dims within 8 stand in the order 0 4 1 5 2 6 3 7 in both Q and K:
+// multiplied one after the other, at twice the products: 4 x 2048 prompt rows are
+// 1.2e-6 off (fp32 sums 5.5e-7), most of it the sums of O.  Dims within 8 stand in the order 0 4 1 5 2 6 3 7 in both Q and K:
 // the order in which a code word's nibbles come out in pairs.
 //
 // Roles: warps 0-3 and 4-7 the softmax of tile 0 and 1 (a thread is a row),
@@ -26,11 +26,11 @@
 // (kept where the rows of the output will stand) and starts anew.
 //
 // Bound: 4 x 128 x 128 x HD multiply-adds a step and tile, 5.2k cycles a step at
-// HD 128; a step takes 8.4k (a tile's softmax and products follow one another)
-// and a CTA 27k beside its steps.  Four prompts of 2048 tokens (32 query, 8 KV
-// heads of 128): 466 us, 295 TFLOP/s of the algorithm's operations, tensor cores
-// busy 0.44 of the time.  Every wait is bounded; a role that gives up raises a
-// flag, and all stop.
+// HD 128; a step takes 8.5k to 9.1k (a tile's softmax and products follow one
+// another), 9.3k with the fp32 sums of O among 16, and a CTA 29k beside its steps.
+// Four prompts of 2048 tokens (32 query, 8 KV heads of 128): 478 us, 287 TFLOP/s of
+// the algorithm's operations, tensor pipe active 0.31 of the time.  Every wait is
+// bounded; a role that gives up raises a flag, and all stop.
 #pragma once
 
 #include <cuda_fp16.h>

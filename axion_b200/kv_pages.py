@@ -2,8 +2,10 @@
 
 One :class:`KVPages` holds the block table and the reference counts of a cache
 of any number of layers and moves page contents in every layer's pool: the
-``k`` and ``v`` tensors of :class:`~axion_b200.paged_kv.PagedKVCache`-like fp16
-or fp32 pages, or the ``pages`` of :class:`~axion_b200.paged_kv.PagedKVCache4`.
+``pages`` of :class:`~axion_b200.paged_kv.PagedKVCache4`, or fp16 or fp32 pages
+``[n_pages, n_kv_heads, 16, head_dim]`` that a caller of the C ABI names in an
+``axkv_cache_t`` with this table (:class:`~axion_b200.paged_kv.PagedKVCache` has
+a table of its own, which does not share pages).
 Everything stays on the device: no call synchronizes or reads back, so serving
 loops can capture them.  Threads may share a table on one stream: a call's
 kernels are launched together.  Invalid entries and a pool without enough free pages
@@ -82,7 +84,9 @@ class KVPages(_DeviceCalls):
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor, tokens: torch.Tensor) -> None:
         """Empty sequence children[i] becomes a copy of the first tokens[i]
-        tokens of parents[i]: full pages shared, a partly filled one copied."""
+        tokens of parents[i]: full pages shared, a partly filled one copied.
+        Appending to either leaves the other as it is; writing again into a
+        shared page (after taking a sequence back) does not."""
         n, at = self._list(parents, children, tokens)
         self._call_ws(self._need + 4 * n, self._lib.axkv_pages_fork, *at, n)
 

@@ -325,7 +325,9 @@ class PagedKVCache4(_DeviceCalls):
         """Causal attention of ragged chunks: rows q_start[i] .. q_start[i + 1] - 1
         of q are sequence q_seq[i] (None: sequence i) at positions q_pos[i] and
         on, at most max_rows of them, their K and V appended.  Rows of no chunk
-        are left as they are in `out` (unset where it is made here)."""
+        are left as they are in `out` (unset where it is made here).  Single rows
+        over long contexts are better off in decode_attention than beside a long
+        prompt here: one kernel takes the whole call, by max_rows."""
         q = self._rows(q, n_heads * self.head_dim, "q")
         n, chunks = q.shape[0], q_pos.shape[0]
         out = self._out(out, q)

@@ -144,8 +144,17 @@ int64_t axkv4_decode_attn_workspace(const axkv4_cache_t* c, int32_t n_rows, int3
  * row with q_pos < 0 attends to nothing and gives zeros (padding of a batch).
  * Pages whose id is outside the pool count as masked and are reported in the
  * status word, as are sequences and positions outside the table.  n_heads a
- * multiple of n_kv_heads, at most 16 times as many; at most 2^20 rows.  The workspace's
- * contents need not be set; calls sharing it must not overlap on the GPU. */
+ * multiple of n_kv_heads, at most 16 times as many; at most 2^20 rows.  q and out
+ * may be the same memory.  The workspace's contents need not be set; calls sharing
+ * it must not overlap on the GPU, and come from one host thread at a time (a call
+ * is two kernels).
+ *
+ * Accuracy: sums, weights and scores are held in fp32, q and the weights enter
+ * the products as two fp16 parts (22 bits).  Relative to its norm a row is off by
+ * 3e-7 to 8e-7 in this call and in short chunks, and by 1e-6 to 2e-6 in long ones
+ * (8e-6 over long contexts of values of one sign, 2.1e-5 where all tokens are
+ * alike), as measured.  A NaN or an infinity in q makes its heads' rows NaN; finite q should
+ * stay below 2^100. */
 int axkv4_decode_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_t n_rows,
                       int32_t n_heads, const int32_t* q_seq, const int32_t* q_pos, float* out,
                       void* workspace, int64_t workspace_bytes, void* stream);
@@ -160,9 +169,16 @@ int64_t axkv4_chunk_attn_workspace(const axkv4_cache_t* c, int32_t n_chunks, int
  * positions q_pos[i], q_pos[i] + 1, ...; each attends to tokens 0 .. its
  * position, their K and V already appended.  q_start (n_chunks + 1 device
  * int32) does not decrease; a chunk has at most max_rows rows (one that has
- * more, or rows outside q, is left out and reported).  At most 65535 chunks of
- * 2^24 rows.  q and out have n_rows rows; rows of no chunk are left as they are in out.  Rows at negative
- * positions give zeros; reports as in axkv4_decode_attn. */
+ * more, or rows outside q, is left out and reported; with max_rows 0 the call
+ * does nothing).  At most 65535 chunks of 2^24 rows.  q and out have n_rows rows
+ * and may be the same memory; rows of no chunk are left as they are in out.
+ * Rows at negative positions give zeros; reports as in axkv4_decode_attn.
+ *
+ * One kernel takes the whole call, by n_chunks and max_rows: the one for long
+ * chunks does not share a chunk's context among SMs.  Single rows over long
+ * contexts belong in an axkv4_decode_attn call of their own rather than beside a
+ * long prompt (15 of them over 16,384 tokens with 2048 prompt rows: 816 us in one
+ * call, 142 + 100 us in two), and max_rows should be near the longest chunk. */
 int axkv4_chunk_attn(const axkv4_cache_t* c, const float* q, int64_t ldq, int32_t n_rows,
                      int32_t n_chunks, int32_t max_rows, int32_t n_heads, const int32_t* q_seq,
                      const int32_t* q_start, const int32_t* q_pos, float* out, void* workspace,
@@ -204,8 +220,11 @@ int axkv_pages_reserve(const axkv_pages_t* p, const int32_t* seqs, const int32_t
 /* Sequence children[i], which holds no page, becomes a copy of the first
  * tokens[i] tokens of parents[i]: full pages are shared, a page that tokens[i]
  * fills in part is copied to a new one.  Shared pages are full, so appending
- * to either sequence leaves the other as it is.  A child is named once in a
- * call and is no parent in it. */
+ * behind those tokens to either sequence leaves the other as it is.  It does not
+ * where a sequence is taken back (rejected draft tokens) to before the last full
+ * page that it shares and written again from there: the pages are not copied on
+ * a write.  Fork it at the shorter length instead, and free the old one.  A child
+ * is named once in a call and is no parent in it. */
 int axkv_pages_fork(const axkv_pages_t* p, const int32_t* parents, const int32_t* children,
                     const int32_t* tokens, int32_t n, void* workspace, int64_t workspace_bytes,
                     void* stream);
